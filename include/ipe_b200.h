@@ -61,7 +61,8 @@ enum {
 const char* ipe_last_error(void);
 int ipe_abi_version(void);
 /* Reads (and with reset != 0 clears) the device error word of the current device: 0 = none,
- * 1 = token ID out of range, 2 = cache position out of range, 3 = a bounded wait timed out.
+ * 1 = token ID out of range, 2 = cache position out of range, 3 = a bounded wait timed out,
+ * 5 = a page ID outside a paged cache.
  * Synchronises the device. */
 int ipe_device_error(int reset, int* out_code);
 
@@ -235,6 +236,54 @@ int ipe_decode_attention_static_scratch(const void* q, const void* k_cache, cons
 int ipe_prefill_attention(const void* q, const void* k_cache, const void* v_cache, void* out,
                           int batch, int q_heads, int kv_heads, int tokens, int capacity,
                           void* stream);
+
+/* ------------------------------------------------------------------ paged cache
+ * Keys and values in pages, for batches of sequences of different lengths. k_pages / v_pages are bf16
+ * [num_pages, kv_heads, page_size, 128] with page_size 16, 32, 64 or 128; position p of sequence s is row
+ * p % page_size of page page_table[s, p / page_size], page_table int32 [sequences, max_pages] (entries past a
+ * sequence's last page are never read). New tokens are ragged: sequence s brings rows cu_tokens[s] ..
+ * cu_tokens[s + 1] - 1 (int32 [sequences + 1]), the last ones of its lengths[s] positions (int32 [sequences]).
+ * Rows behind the last sequence are left as they are. 1 to 8 query heads per KV head.
+ *
+ * The integers are read on the device only, so a captured call replays with other values. A length that is
+ * negative, larger than max_pages * page_size or less than the sequence's new tokens sets device error 2, a page
+ * outside [0, num_pages) device error 5; such a sequence's output rows hold no meaning, the others are served and
+ * nothing outside the buffers is touched. Outputs must not overlap inputs. */
+
+/* ipe_qk_norm_rope_append (src/ipe/forward.py:101-109) for a ragged batch and a paged cache: token i of the n
+ * that a sequence brings is at position lengths[s] - n + i. Computed in fp32 and rounded to bf16 once.
+ *   qkv      bf16 [tokens, (q_heads + 2*kv_heads) * 128]   (q | k | v per token)
+ *   cos/sin  [table_rows, 128] by position, bf16 (table_dtype 0) or fp32 (1); a position past them sets device
+ *            error 2 and its row is skipped
+ *   q_out    bf16 [tokens, q_heads, 128] */
+int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, int kv_heads,
+                                  const void* q_norm_weight, const void* k_norm_weight, const void* cos_table,
+                                  const void* sin_table, int table_dtype, int64_t table_rows,
+                                  const int32_t* cu_tokens, const int32_t* lengths, const int32_t* page_table,
+                                  int sequences, int max_pages, void* q_out, void* k_pages, void* v_pages,
+                                  int64_t num_pages, int page_size, float eps, void* stream);
+
+/* One query token per sequence, q bf16 [sequences, q_heads, 128], over keys 0 .. lengths[s] - 1: out bf16
+ * [sequences, q_heads * 128] (src/ipe/ops.py:78-101, decode). Length 0 gives zeros. */
+int ipe_paged_decode_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                               const int32_t* lengths, void* out, int sequences, int q_heads, int kv_heads,
+                               int64_t num_pages, int page_size, int max_pages, void* stream);
+
+/* Causal attention of ragged new tokens, q bf16 [tokens, q_heads, 128]: token i of the n that sequence s brings
+ * sees keys 0 .. lengths[s] - n + i. out bf16 [tokens, q_heads * 128] (src/ipe/ops.py:78-101, causal). */
+int ipe_paged_prefill_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                                const int32_t* cu_tokens, const int32_t* lengths, void* out, int64_t tokens,
+                                int sequences, int q_heads, int kv_heads, int64_t num_pages, int page_size,
+                                int max_pages, void* stream);
+
+/* ipe_paged_decode_attention of sequences that begin with the same pages: positions below prefix_count *
+ * page_size of every sequence are in prefix_pages (int32 [prefix_count], prefix_count <= max_pages), whose keys
+ * are read once for the batch; page_table is read for the positions behind them alone. lengths count the prefix;
+ * a sequence that ends inside it sees its own lengths[s] keys of it. */
+int ipe_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* prefix_pages,
+                                int prefix_count, const int32_t* page_table, const int32_t* lengths, void* out,
+                                int sequences, int q_heads, int kv_heads, int64_t num_pages, int page_size,
+                                int max_pages, void* stream);
 
 /* ------------------------------------------------------------------ tensor-core GEMM */
 

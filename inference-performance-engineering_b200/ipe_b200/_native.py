@@ -46,6 +46,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ipe_decode_attention_qkv_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),
     "ipe_decode_attention_static_scratch": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P, _P]),
     "ipe_prefill_attention": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
+    "ipe_paged_qk_norm_rope_append": (c_int, [_P, c_int64, c_int, c_int, _P, _P, _P, _P, c_int, c_int64, _P, _P, _P, c_int,
+                                              c_int, _P, _P, _P, c_int64, c_int, c_float, _P]),
+    "ipe_paged_decode_attention": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int, c_int, _P]),
+    "ipe_paged_prefill_attention": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int64, c_int,
+                                            c_int, _P]),
+    "ipe_shared_prefix_attention": (c_int, [_P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int,
+                                            c_int, _P]),
     "ipe_gemm": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P]),
     "ipe_decode_step": (c_int, [ctypes.c_void_p, _P]),
     "ipe_decode_step_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),

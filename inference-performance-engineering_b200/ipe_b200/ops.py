@@ -19,6 +19,9 @@ Operators and the reference code each replaces (src/ipe/...):
   sample_logits           engine.py:28-41 (logits the caller holds)
   decode_tiles            (no counterpart) the decode-side weight layout the decode linears read
   gemm                    the prefill F.linear calls of forward.py:100-115 and forward.py:145-152
+
+The operators over a paged cache (paged_qk_norm_rope_append, paged_decode_attention,
+paged_prefill_attention, shared_prefix_attention) are in ipe_b200.paged and offered here too.
 """
 
 from __future__ import annotations
@@ -26,6 +29,8 @@ from __future__ import annotations
 import torch
 
 from ipe_b200 import _native as nat
+from ipe_b200.paged import (paged_decode_attention, paged_prefill_attention, paged_qk_norm_rope_append,
+                            shared_prefix_attention)
 
 
 def _stream() -> int:
@@ -288,6 +293,15 @@ _lib.define("decode_attention(Tensor q, Tensor k_cache, Tensor v_cache, int leng
 _lib.define("prefill_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor(a!) out) -> ()")
 _lib.define("lm_head_sample(Tensor x, Tensor norm_weight, Tensor lm_tiles, float eps, float temperature, int seed, "
             "Tensor(a!) logits) -> (Tensor, Tensor)")
+_lib.define("paged_qk_norm_rope_append(Tensor qkv, Tensor q_norm, Tensor k_norm, Tensor cos, Tensor sin, "
+            "Tensor cu_tokens, Tensor lengths, Tensor page_table, float eps, Tensor(a!) q_out, Tensor(b!) k_pages, "
+            "Tensor(c!) v_pages) -> ()")
+_lib.define("paged_decode_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor lengths, "
+            "Tensor(a!) out) -> ()")
+_lib.define("paged_prefill_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor cu_tokens, "
+            "Tensor lengths, Tensor(a!) out) -> ()")
+_lib.define("shared_prefix_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor prefix_pages, Tensor page_table, "
+            "Tensor lengths, Tensor(a!) out) -> ()")
 
 
 def _op_rms_norm(x, weight, eps, out):
@@ -321,5 +335,9 @@ def _returns_none(fn):
 
 for _name, _fn in (("rmsnorm_qkv", rmsnorm_qkv), ("linear_residual", linear_residual),
                    ("rmsnorm_gate_up_silu", rmsnorm_gate_up_silu), ("qk_norm_rope_append", qk_norm_rope_append),
-                   ("decode_attention", decode_attention), ("prefill_attention", prefill_attention)):
+                   ("decode_attention", decode_attention), ("prefill_attention", prefill_attention),
+                   ("paged_qk_norm_rope_append", paged_qk_norm_rope_append),
+                   ("paged_decode_attention", paged_decode_attention),
+                   ("paged_prefill_attention", paged_prefill_attention),
+                   ("shared_prefix_attention", shared_prefix_attention)):
     _lib.impl(_name, _returns_none(_fn), "CUDA")

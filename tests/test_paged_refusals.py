@@ -1,0 +1,65 @@
+"""What the paged-cache operators refuse on the host, without a GPU: the C entry points reject bad sizes and pointers
+before any device call, and the Python functions reject wrong devices, types, shapes and strides."""
+
+import pytest
+import torch
+
+from ipe_b200 import _native as nat
+from ipe_b200 import ops
+
+GOOD = {
+    "ipe_paged_qk_norm_rope_append": dict(qkv=16, tokens=4, q_heads=16, kv_heads=8, q_norm=16, k_norm=16, cos=16, sin=16,
+                                          table_dtype=0, table_rows=64, cu_tokens=16, lengths=16, page_table=16, sequences=2,
+                                          max_pages=4, q_out=16, k_pages=16, v_pages=16, num_pages=9, page_size=16, eps=1e-6,
+                                          stream=None),
+}
+
+BAD = [
+    ("ipe_paged_qk_norm_rope_append", dict(q_heads=15)),
+    ("ipe_paged_qk_norm_rope_append", dict(q_heads=72)),
+    ("ipe_paged_qk_norm_rope_append", dict(kv_heads=0)),
+    ("ipe_paged_qk_norm_rope_append", dict(page_size=24)),
+    ("ipe_paged_qk_norm_rope_append", dict(page_size=256)),
+    ("ipe_paged_qk_norm_rope_append", dict(num_pages=0)),
+    ("ipe_paged_qk_norm_rope_append", dict(num_pages=2 ** 24)),
+    ("ipe_paged_qk_norm_rope_append", dict(max_pages=0)),
+    ("ipe_paged_qk_norm_rope_append", dict(max_pages=2 ** 27)),
+    ("ipe_paged_qk_norm_rope_append", dict(tokens=-1)),
+    ("ipe_paged_qk_norm_rope_append", dict(tokens=2 ** 31)),
+    ("ipe_paged_qk_norm_rope_append", dict(sequences=-1)),
+    ("ipe_paged_qk_norm_rope_append", dict(table_dtype=2)),
+    ("ipe_paged_qk_norm_rope_append", dict(table_rows=0)),
+] + [("ipe_paged_qk_norm_rope_append", {p: v}) for p in
+     ("qkv", "q_norm", "k_norm", "cos", "sin", "cu_tokens", "lengths", "page_table", "q_out", "k_pages", "v_pages")
+     for v in (None, 18)]
+
+
+@pytest.mark.parametrize(("name", "change"), BAD)
+def test_the_entry_points_refuse(name, change):
+    args = {**GOOD[name], **change}
+    assert getattr(nat.load(), name)(*args.values()) in (1, 2)
+    assert nat.load().ipe_last_error().decode().startswith(name)
+
+
+def test_nothing_to_do_is_no_error():
+    name = "ipe_paged_qk_norm_rope_append"
+    for change in (dict(tokens=0, qkv=None, q_out=None), dict(sequences=0, page_table=None)):
+        assert getattr(nat.load(), name)(*{**GOOD[name], **change}.values()) == 0
+
+
+def test_cpu_tensors_are_refused():
+    pages, table, one = torch.zeros(3, 2, 16, 128, dtype=torch.bfloat16), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q, out, cu = torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.zeros(1, 512, dtype=torch.bfloat16), torch.tensor([0, 1], dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_decode_attention(q, pages, pages, table, one, out)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_prefill_attention(q, pages, pages, table, cu, one, out)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.shared_prefix_attention(q, pages, pages, one, table, one, out)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_qk_norm_rope_append(q, q, q, q, q, cu, one, table, 1e-6, q, pages, pages)
+
+
+def test_the_operators_are_registered():
+    for name in ("paged_qk_norm_rope_append", "paged_decode_attention", "paged_prefill_attention", "shared_prefix_attention"):
+        assert hasattr(torch.ops.ipe_b200, name)
