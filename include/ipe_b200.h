@@ -264,10 +264,13 @@ int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, 
                                   int64_t num_pages, int page_size, float eps, void* stream);
 
 /* One query token per sequence, q bf16 [sequences, q_heads, 128], over keys 0 .. lengths[s] - 1: out bf16
- * [sequences, q_heads * 128] (src/ipe/ops.py:78-101, decode). Length 0 gives zeros. */
+ * [sequences, q_heads * 128] (src/ipe/ops.py:78-101, decode). Length 0 gives zeros. The workspace is 256-byte
+ * aligned, of any contents, and belongs to the call until it has run. */
 int ipe_paged_decode_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                const int32_t* lengths, void* out, int sequences, int q_heads, int kv_heads,
-                               int64_t num_pages, int page_size, int max_pages, void* stream);
+                               int64_t num_pages, int page_size, int max_pages, void* workspace,
+                               size_t workspace_bytes, void* stream);
+size_t ipe_paged_decode_attention_workspace(int sequences, int q_heads, int kv_heads);
 
 /* Causal attention of ragged new tokens, q bf16 [tokens, q_heads, 128]: token i of the n that sequence s brings
  * sees keys 0 .. lengths[s] - n + i. out bf16 [tokens, q_heads * 128] (src/ipe/ops.py:78-101, causal). */

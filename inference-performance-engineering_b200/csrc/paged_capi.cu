@@ -65,9 +65,20 @@ int rows_checks(const char* name, const void* q, const void* out) {
   return IPE_OK;
 }
 
+int workspace_checks(const char* name, const void* workspace, size_t bytes, size_t need) {
+  if (need > 0 && (!workspace || misaligned(workspace, 256) || bytes < need))
+    return fail(IPE_ERR_ARGUMENT, "%s: a 256-byte aligned workspace of %zu bytes is needed", name, need);
+  return IPE_OK;
+}
+
 }  // namespace
 
 extern "C" {
+
+size_t ipe_paged_decode_attention_workspace(int sequences, int q_heads, int kv_heads) {
+  if (sequences < 1 || kv_heads < 1 || q_heads < kv_heads) return 0;
+  return ipe::paged_decode_workspace_bytes(sequences, q_heads, kv_heads);
+}
 
 int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, int kv_heads,
                                   const void* q_norm_weight, const void* k_norm_weight, const void* cos_table,
@@ -97,7 +108,8 @@ int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, 
 
 int ipe_paged_decode_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                const int32_t* lengths, void* out, int sequences, int q_heads, int kv_heads,
-                               int64_t num_pages, int page_size, int max_pages, void* stream) {
+                               int64_t num_pages, int page_size, int max_pages, void* workspace,
+                               size_t workspace_bytes, void* stream) {
   const char* name = "ipe_paged_decode_attention";
   ipe::PagedCache c;
   if (int status = paged_cache(name, k_pages, v_pages, page_table, lengths, sequences, sequences, q_heads, kv_heads,
@@ -105,8 +117,10 @@ int ipe_paged_decode_attention(const void* q, const void* k_pages, const void* v
     return status;
   if (sequences == 0) return IPE_OK;
   if (int status = rows_checks(name, q, out)) return status;
-  return finish(ipe::launch_paged_attention(c, q, k_pages, v_pages, out, sequences, q_heads,
-                                            static_cast<cudaStream_t>(stream)),
+  const size_t need = ipe::paged_decode_workspace_bytes(sequences, q_heads, kv_heads);
+  if (int status = workspace_checks(name, workspace, workspace_bytes, need)) return status;
+  return finish(ipe::launch_paged_decode(c, q, k_pages, v_pages, out, q_heads, workspace,
+                                         static_cast<cudaStream_t>(stream)),
                 name);
 }
 

@@ -1,0 +1,370 @@
+// Decode attention over a paged cache: one query token per sequence, G = 1..8 query heads per KV head.
+//
+// Bound by memory: every key and value byte is read once for the G heads that share it. The batch's
+// keys are cut into units of 64 keys of one (sequence, KV head), in that order, and the units are dealt
+// to the CTAs in equal contiguous runs, so a batch with one long sequence keeps every SM as busy as an
+// even one. A run's first and last piece may be part of an item; parts go to the workspace as records
+// (unnormalised o, maximum, sum) that a second kernel merges in order of the keys.
+//
+// In a unit each of the 4 warps has 16 keys and a running softmax of its own; the warps meet once per
+// piece. S = K q^T and O^T = V^T P^T as m16n8k16 products with the keys (then the head's dimensions) as
+// the 16 rows and the query heads as the 8 columns, so a thread's scores and its output accumulators
+// belong to the same two heads. P enters as two bf16 terms (value and remainder), so the weights keep
+// 16 bits: the products are idle anyway. K and V come through per-warp rings of cp.async copies, which
+// fill keys past the sequence's end with zeros without reading them: what an unused row holds (NaN,
+// say) never meets a weight of zero.
+#include <algorithm>
+
+#include "launch.h"
+#include "paged.cuh"
+#include "tensor_map.h"
+
+namespace ipe {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnit = 16 * kWarps;       // keys
+constexpr int kStages = 3;               // units in flight per CTA
+constexpr int kStageBytes = 2 * 16 * 256;  // one warp's keys and values of a unit
+constexpr int kCtasPerSm = 2;
+constexpr int kHeads = 8;                // columns of the products
+constexpr int kMergeStride = 132;        // floats; spreads a warp's 4 head pairs over the banks
+constexpr int kRecord = 132;             // floats: o[128], maximum, sum, 2 unused
+constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // 128^-0.5 * log2(e)
+constexpr size_t kSmem = static_cast<size_t>(kStages) * kWarps * kStageBytes +
+                         static_cast<size_t>(kWarps) * kHeads * kMergeStride * sizeof(float);
+
+struct DecodeArgs {
+  PagedCache c;
+  const bf16* q;
+  const bf16* k;
+  const bf16* v;
+  bf16* out;
+  float* records;    // [grid][2][G][kRecord]
+  int64_t* offsets;  // [sequences + 1]: units of one KV head before each sequence
+  int q_heads;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ int units_of(const PagedCache& c, int s) { return (c.length(s) + kUnit - 1) / kUnit; }
+
+// The units are dealt to `runs` CTAs, none of them without one; run r begins with unit run_start(r).
+__device__ __forceinline__ int runs_of(int64_t units, int ctas) { return units < ctas ? static_cast<int>(units) : ctas; }
+__device__ __forceinline__ int64_t run_start(int64_t units, int run, int runs) { return units * run / max(runs, 1); }
+
+// A place in the batch's sequence of units.
+struct Cursor {
+  int s, h, unit, units, length;
+  __device__ __forceinline__ void advance(const PagedCache& c) {
+    if (++unit < units) return;
+    unit = 0;
+    if (++h < c.kv_heads) return;
+    h = 0;
+    do {
+      ++s;
+      length = s < c.sequences ? c.length(s) : kUnit;
+      units = (length + kUnit - 1) / kUnit;
+    } while (units == 0);
+  }
+};
+
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(const DecodeArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t warp_units[kWarps];
+  __shared__ Cursor start;
+  __shared__ float stats[kWarps][kHeads][2];
+  float* merge = reinterpret_cast<float*>(smem + static_cast<size_t>(kStages) * kWarps * kStageBytes);
+  const PagedCache& c = a.c;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.q_heads / c.kv_heads;
+  pdl_trigger();
+
+  // ------------------------------------------------------------------ this CTA's run of units
+  const int per = (c.sequences + kThreads - 1) / kThreads;
+  const int s_lo = min(c.sequences, static_cast<int>(threadIdx.x) * per), s_hi = min(c.sequences, s_lo + per);
+  int64_t mine = 0;
+  for (int s = s_lo; s < s_hi; ++s) mine += units_of(c, s);
+  int64_t scan = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += up;
+  }
+  if (lane == 31) warp_units[warp] = scan;
+  __syncthreads();
+  int64_t before = scan - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += warp_units[w];
+    total += warp_units[w];
+  }
+  const int64_t units = total * c.kv_heads;
+  const int runs = runs_of(units, gridDim.x);
+  const int64_t u0 = run_start(units, blockIdx.x, runs), u1 = run_start(units, blockIdx.x + 1, runs);
+  for (int s = s_lo; s < s_hi; ++s) {
+    const int n = units_of(c, s);
+    if (blockIdx.x == 0) a.offsets[s] = before;
+    if (n > 0 && u0 >= before * c.kv_heads && u0 < (before + n) * c.kv_heads) {
+      const int r = static_cast<int>(u0 - before * c.kv_heads);
+      start = Cursor{s, r / n, r % n, n, c.length(s)};
+    }
+    if (n == 0 && s % gridDim.x == blockIdx.x) {  // no keys: zeros
+      uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(s) * a.q_heads * 128);
+      for (int i = 0; i < a.q_heads * 16; ++i) row[i] = make_uint4(0, 0, 0, 0);
+    }
+    before += n;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[c.sequences] = total;
+  __syncthreads();
+  if (blockIdx.x >= runs) return;
+  const int64_t count = u1 - u0;
+
+  // ------------------------------------------------------------------ loads
+  const uint32_t ring = smem_addr(smem) + warp * kStageBytes;  // stage i at + i * kWarps * kStageBytes
+  Cursor ahead = start;
+  int64_t issued = 0;
+  int page = 0;  // of `ahead`
+  auto look_up = [&] {
+    const int key0 = ahead.unit * kUnit + warp * 16;
+    page = key0 < ahead.length ? c.page(ahead.s, key0) : 0;
+  };
+  auto issue = [&](int stage) {
+    if (issued < count) {
+      const int key0 = ahead.unit * kUnit + warp * 16;
+      const int valid = ahead.length - key0;  // keys of these 16 that exist
+      const int64_t row0 = c.page_row(page, ahead.h) + (key0 & (c.page_size() - 1));
+      const int chunk = lane & 15;
+      const uint32_t dst = ring + stage * (kWarps * kStageBytes);
+      const bf16* ks = a.k + row0 * 128 + chunk * 8;
+      const bf16* vs = a.v + row0 * 128 + chunk * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = (lane >> 4) + 2 * i;
+        const uint32_t at = row * 256 + ((chunk ^ (row & 7)) << 4);
+        const bool real = row < valid;
+        cp_async16(dst + at, real ? ks + row * 128 : a.k, real ? 16 : 0);
+        cp_async16(dst + 4096 + at, real ? vs + row * 128 : a.v, real ? 16 : 0);
+      }
+      if (++issued < count) {
+        ahead.advance(c);
+        look_up();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  look_up();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+  // ------------------------------------------------------------------ products
+  Cursor at = start;
+  uint32_t qb[8][2];  // q^T of this piece: k = 16 kk + 2 (lane % 4) (+ 8), n = lane / 4
+  float acc[8][4];    // O^T: rows 16 t + lane / 4 (+ 8), heads 2 (lane % 4) (+ 1)
+  float m[2], l[2];
+  bool fresh = true, first_piece = true, whole_start = true;
+  const int frow = (lane & 7) + ((lane >> 3) & 1) * 8, fcol = lane >> 4;  // K fragments
+  const int trow = (lane & 7) + (lane >> 4) * 8, tcol = (lane >> 3) & 1;  // V fragments, transposed
+  int stage = 0;
+  for (int64_t u = 0; u < count; ++u) {
+    issue(stage == 0 ? kStages - 1 : stage - 1);
+    if (fresh) {
+      fresh = false;
+      whole_start = at.unit == 0;
+      const bf16* qr = a.q + (static_cast<int64_t>(at.s) * a.q_heads + at.h * group + (lane >> 2)) * 128 + 2 * (lane & 3);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const bool real = (lane >> 2) < group;
+        qb[kk][0] = real ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk) : 0u;
+        qb[kk][1] = real ? *reinterpret_cast<const uint32_t*>(qr + 16 * kk + 8) : 0u;
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const uint32_t ks = ring + stage * (kWarps * kStageBytes), vs = ks + 4096;
+    float sc[2][4] = {};
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      uint32_t f0, f1, f2, f3;
+      ldmatrix_x4(f0, f1, f2, f3, ks + frow * 256 + (((2 * kk + fcol) ^ (frow & 7)) << 4));
+      mma16816(sc[kk & 1], f0, f1, f2, f3, qb[kk][0], qb[kk][1]);
+    }
+    const int key = at.unit * kUnit + warp * 16 + (lane >> 2);
+    float s4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s4[i] = key + (i >> 1) * 8 < at.length ? sc[0][i] + sc[1][i] : -INFINITY;
+    float keep[2], p[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float top = fmaxf(s4[e], s4[2 + e]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = fmaxf(top, m[e]);
+      const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
+      keep[e] = exp2_approx(m[e] * kScaleLog2 - base);
+      m[e] = top;
+      p[e] = exp2_approx(s4[e] * kScaleLog2 - base);
+      p[2 + e] = exp2_approx(s4[2 + e] * kScaleLog2 - base);
+      l[e] = l[e] * keep[e] + p[e] + p[2 + e];
+    }
+    const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1])), b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
+    const uint32_t r0 = transpose8x8(pack_bf16x2(p[0] - bf16_round(p[0]), p[1] - bf16_round(p[1])));
+    const uint32_t r1 = transpose8x8(pack_bf16x2(p[2] - bf16_round(p[2]), p[3] - bf16_round(p[3])));
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      uint32_t f0, f1, f2, f3;
+      ldmatrix_x4_trans(f0, f1, f2, f3, vs + trow * 256 + (((2 * t + tcol) ^ (trow & 7)) << 4));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] *= keep[i & 1];
+      mma16816(acc[t], f0, f1, f2, f3, b0, b1);
+      mma16816(acc[t], f0, f1, f2, f3, r0, r1);
+    }
+    __syncwarp();
+    if (++stage == kStages) stage = 0;
+
+    if (at.unit + 1 == at.units || u + 1 == count) {  // the piece ends: the warps meet
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], o);
+        const int g = 2 * (lane & 3) + e;
+        if (lane < 4) {
+          stats[warp][g][0] = m[e];
+          stats[warp][g][1] = l[e];
+        }
+        float* o = merge + (warp * kHeads + g) * kMergeStride + (lane >> 2);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          o[16 * t] = acc[t][e];
+          o[16 * t + 8] = acc[t][2 + e];
+        }
+      }
+      __syncthreads();
+      const bool whole = whole_start && at.unit + 1 == at.units;
+      const int slot = first_piece ? 0 : 1;
+      first_piece = false;
+      for (int g = 0; g < group; ++g) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stats[w][g][0]);
+        const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
+        float sum = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float e = exp2_approx(stats[w][g][0] * kScaleLog2 - base);
+          sum += e * stats[w][g][1];
+          o += e * merge[(w * kHeads + g) * kMergeStride + threadIdx.x];
+        }
+        if (whole) {
+          a.out[(static_cast<int64_t>(at.s) * a.q_heads + at.h * group + g) * 128 + threadIdx.x] = __float2bfloat16_rn(o / sum);
+        } else {
+          float* rec = a.records + ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * group + g) * kRecord;
+          rec[threadIdx.x] = o;
+          if (threadIdx.x == 0) {
+            rec[128] = top;
+            rec[129] = sum;
+          }
+        }
+      }
+      __syncthreads();
+      fresh = true;
+    }
+    if (u + 1 < count) at.advance(c);
+  }
+}
+
+// One warp per (sequence, query head) whose units lie in more than one run: merges the runs' records.
+__global__ void __launch_bounds__(kThreads) paged_decode_merge_kernel(const DecodeArgs a, int ctas) {
+  pdl_wait();
+  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  const PagedCache& c = a.c;
+  if (warp >= static_cast<int64_t>(c.sequences) * a.q_heads) return;
+  const int lane = threadIdx.x & 31;
+  const int s = static_cast<int>(warp / a.q_heads), head = static_cast<int>(warp % a.q_heads);
+  const int group = a.q_heads / c.kv_heads, h = head / group, g = head % group;
+  const int64_t from = __ldcg(a.offsets + s), n = __ldcg(a.offsets + s + 1) - from;
+  const int64_t units = __ldcg(a.offsets + c.sequences) * c.kv_heads;
+  if (n == 0) return;  // zeros, already written
+  const int runs = runs_of(units, ctas);
+  const int64_t first = from * c.kv_heads + h * n;  // the item's units: first .. first + n - 1
+  const int run_lo = static_cast<int>(((first + 1) * runs - 1) / units);
+  const int run_hi = static_cast<int>(((first + n) * runs - 1) / units);
+  if (run_lo == run_hi) return;  // whole, already written
+  // a run's first piece is its slot 0: that of every run after the first, and of the first if it begins with the item
+  const int slot_lo = run_start(units, run_lo, runs) == first ? 0 : 1;
+  auto record = [&](int run) {
+    return a.records + ((static_cast<int64_t>(run) * 2 + (run == run_lo ? slot_lo : 0)) * group + g) * kRecord;
+  };
+  float top = -INFINITY;
+  for (int r = run_lo + lane; r <= run_hi; r += 32) top = fmaxf(top, __ldcg(record(r) + 128));
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int r = run_lo; r <= run_hi; ++r) {
+    const float* rec = record(r);
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
+    const float e = exp2_approx(__ldcg(rec + 128) * kScaleLog2 - base);
+    sum += e * __ldcg(rec + 129);
+    o.x += e * x.x;
+    o.y += e * x.y;
+    o.z += e * x.z;
+    o.w += e * x.w;
+  }
+  const float inv = 1.f / sum;
+  *reinterpret_cast<uint2*>(a.out + warp * 128 + lane * 4) =
+      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+}
+
+size_t offsets_bytes(int sequences) { return ((static_cast<size_t>(sequences) + 1) * sizeof(int64_t) + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t paged_decode_workspace_bytes(int sequences, int q_heads, int kv_heads) {
+  return offsets_bytes(sequences) + static_cast<size_t>(kCtasPerSm * sm_count()) * 2 * (q_heads / kv_heads) * kRecord * sizeof(float);
+}
+
+cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
+                                int q_heads, void* workspace, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(kSmem));
+  if (e != cudaSuccess) return e;
+  DecodeArgs a{};
+  a.c = c;
+  a.q = static_cast<const bf16*>(q);
+  a.k = static_cast<const bf16*>(k_pages);
+  a.v = static_cast<const bf16*>(v_pages);
+  a.out = static_cast<bf16*>(out);
+  a.offsets = static_cast<int64_t*>(workspace);
+  a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + offsets_bytes(c.sequences));
+  a.q_heads = q_heads;
+  const int64_t capacity = static_cast<int64_t>(c.max_pages) << c.page_shift;
+  const int64_t most = static_cast<int64_t>(c.sequences) * c.kv_heads * ((capacity + kUnit - 1) / kUnit);
+  const int grid = static_cast<int>(std::min<int64_t>(kCtasPerSm * sm_count(), most));
+  paged_decode_kernel<<<grid, kThreads, kSmem, stream>>>(a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || capacity <= kUnit) return e;  // one unit per item: nothing to merge
+  const int64_t warps = static_cast<int64_t>(c.sequences) * q_heads;
+  return launch_pdl(paged_decode_merge_kernel, dim3(static_cast<unsigned>((warps + kWarps - 1) / kWarps)), dim3(kThreads),
+                    0, stream, a, grid);
+}
+
+}  // namespace ipe

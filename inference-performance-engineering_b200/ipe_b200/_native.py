@@ -48,7 +48,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ipe_prefill_attention": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "ipe_paged_qk_norm_rope_append": (c_int, [_P, c_int64, c_int, c_int, _P, _P, _P, _P, c_int, c_int64, _P, _P, _P, c_int,
                                               c_int, _P, _P, _P, c_int64, c_int, c_float, _P]),
-    "ipe_paged_decode_attention": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int, c_int, _P]),
+    "ipe_paged_decode_attention": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int, c_int, _P,
+                                           c_size_t, _P]),
+    "ipe_paged_decode_attention_workspace": (c_size_t, [c_int, c_int, c_int]),
     "ipe_paged_prefill_attention": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int64, c_int,
                                             c_int, _P]),
     "ipe_shared_prefix_attention": (c_int, [_P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int,

@@ -26,6 +26,7 @@ Every function runs on the current stream of its tensors' device. Outputs must n
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 
@@ -73,6 +74,16 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(entry: str, device_index: int, *sizes: int) -> int:
+    return int(getattr(nat.load(), entry)(*sizes))
+
+
+def _workspace(device: torch.device, entry: str, *sizes: int) -> torch.Tensor:
+    """The call's own scratch, from torch's allocator: calls on other streams, and captured ones, have others."""
+    return torch.empty(_workspace_bytes(entry, device.index, *sizes), dtype=torch.uint8, device=device)
+
+
 def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor,
                               sin: torch.Tensor, cu_tokens: torch.Tensor, lengths: torch.Tensor,
                               page_table: torch.Tensor, eps: float, q_out: torch.Tensor, k_pages: torch.Tensor,
@@ -115,9 +126,10 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
     q_heads = _heads(name, q, out, sequences)
     with _on(device):
+        ws = _workspace(device, "ipe_paged_decode_attention_workspace", sequences, q_heads, kv_heads)
         nat.call("ipe_paged_decode_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                  page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), sequences, q_heads, kv_heads, pages,
-                 page_size, width, _stream(device))
+                 page_size, width, ws.data_ptr(), ws.numel(), _stream(device))
     return out
 
 
