@@ -277,7 +277,8 @@ size_t ipe_paged_decode_attention_workspace(int sequences, int q_heads, int kv_h
 int ipe_paged_prefill_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                 const int32_t* cu_tokens, const int32_t* lengths, void* out, int64_t tokens,
                                 int sequences, int q_heads, int kv_heads, int64_t num_pages, int page_size,
-                                int max_pages, void* stream);
+                                int max_pages, void* workspace, size_t workspace_bytes, void* stream);
+size_t ipe_paged_prefill_attention_workspace(int64_t tokens, int sequences, int q_heads, int kv_heads);
 
 /* ipe_paged_decode_attention of sequences that begin with the same pages: positions below prefix_count *
  * page_size of every sequence are in prefix_pages (int32 [prefix_count], prefix_count <= max_pages), whose keys

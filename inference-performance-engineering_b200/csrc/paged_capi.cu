@@ -80,6 +80,11 @@ size_t ipe_paged_decode_attention_workspace(int sequences, int q_heads, int kv_h
   return ipe::paged_decode_workspace_bytes(sequences, q_heads, kv_heads);
 }
 
+size_t ipe_paged_prefill_attention_workspace(int64_t tokens, int sequences, int q_heads, int kv_heads) {
+  if (tokens < 1 || sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8) return 0;
+  return ipe::paged_prefill_workspace_bytes(tokens, sequences, q_heads, kv_heads);
+}
+
 int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, int kv_heads,
                                   const void* q_norm_weight, const void* k_norm_weight, const void* cos_table,
                                   const void* sin_table, int table_dtype, int64_t table_rows,
@@ -127,7 +132,7 @@ int ipe_paged_decode_attention(const void* q, const void* k_pages, const void* v
 int ipe_paged_prefill_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                 const int32_t* cu_tokens, const int32_t* lengths, void* out, int64_t tokens,
                                 int sequences, int q_heads, int kv_heads, int64_t num_pages, int page_size,
-                                int max_pages, void* stream) {
+                                int max_pages, void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "ipe_paged_prefill_attention";
   ipe::PagedCache c;
   if (int status = paged_cache(name, k_pages, v_pages, page_table, lengths, tokens, sequences, q_heads, kv_heads,
@@ -137,8 +142,10 @@ int ipe_paged_prefill_attention(const void* q, const void* k_pages, const void* 
   if (int status = rows_checks(name, q, out)) return status;
   if (!cu_tokens || misaligned(cu_tokens, 4)) return fail(IPE_ERR_ARGUMENT, "%s: cu_tokens", name);
   c.cu_tokens = cu_tokens;
-  return finish(ipe::launch_paged_attention(c, q, k_pages, v_pages, out, tokens, q_heads,
-                                            static_cast<cudaStream_t>(stream)),
+  const size_t need = ipe::paged_prefill_workspace_bytes(tokens, sequences, q_heads, kv_heads);
+  if (int status = workspace_checks(name, workspace, workspace_bytes, need)) return status;
+  return finish(ipe::launch_paged_prefill(c, q, k_pages, v_pages, out, tokens, q_heads, workspace,
+                                          static_cast<cudaStream_t>(stream)),
                 name);
 }
 

@@ -1,0 +1,888 @@
+// Causal attention of ragged new tokens over a paged cache, on the 5th-generation tensor cores.
+//
+// A block of work is up to 256 query rows of one (sequence, KV head): two tiles of 128 rows, a row being
+// one of the G query heads of one token (tokens of 128 / G, whole), so the G heads share every key that
+// is read. Per key tile of 128 keys and query tile: S = Q K^T (tcgen05.mma into tensor memory), a row
+// per thread reads its scores, keeps an fp32 running maximum and sum in base 2, writes P over the scores
+// as bf16, and O += P V takes P from tensor memory. The two query tiles take turns: while one's scores
+// are in the softmax warps the tensor cores work on the other's products.
+//
+// P is the one rounding before the output's: weights of 8 bits, whose errors average out over the keys;
+// the sum they are divided by is of the unrounded weights. The running maximum moves only when a row's
+// scores pass it by 2^8 (weights up to 256 are as exact in bf16 and fp32 as weights up to 1), so the
+// accumulator in tensor memory is rescaled a few times per row instead of at every tile.
+//
+// Warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread; warp 8: work list and TMA loads;
+// warp 9: tensor memory and MMA issue. Persistent, one CTA per SM; the blocks go to the CTAs heaviest
+// first, back and forth. Where there are fewer blocks than that can balance, every block's key tiles are
+// dealt to the CTAs in equal contiguous runs instead; parts of a block go to the workspace as records (unnormalised o, maximum, sum),
+// merged by a second kernel in order of the keys.
+//
+// Values past a block's last key are zeroed in shared memory before they meet their zero weights. A row
+// whose accumulator is not finite all the same (a value that is infinite or NaN, its own or one of a
+// later token in the tile) is computed again key by key from the keys it sees.
+// Every mbarrier wait is bounded; a timeout sets the device error word and the CTA winds down.
+#include <algorithm>
+
+#include "launch.h"
+#include "paged.cuh"
+#include "tensor_map.h"
+
+namespace ipe {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;  // warps 0-7: softmax
+constexpr int kBM = 128, kBN = 128, kD = 128;
+constexpr int kHalf = 128 * 64 * 2;  // a 128-row x 64-column bf16 block, 128-byte swizzle
+constexpr int kTile = 2 * kHalf;
+constexpr int kStages = 4;           // K or V tiles in flight
+constexpr int kTmemCols = 512;       // S0 [0, 128), S1 [128, 256), O0 [256, 384), O1 [384, 512)
+constexpr int kMaxListed = 1024;     // sequences (and, in runs, blocks) listed in shared memory
+constexpr int kRecord = 132;         // floats: o[128], maximum, sum, 2 unused
+constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // 128^-0.5 * log2(e)
+constexpr float kSlack = 8.f / kScaleLog2;  // how far scores may pass the maximum in use
+
+struct Work {       // one piece: key tiles of a block
+  int token0;       // first query row's token (row of q)
+  int tokens;       // of the block
+  int position0;    // of token0 in its sequence
+  int sequence;
+  int kv_head;
+  int keys;         // the block's keys: tiles end here
+  int tile0;        // first key tile of the piece
+  int count[2];     // key tiles of each query tile in this piece
+  int record;       // where the piece's rows go: -1 the output, else a record slot
+};
+
+struct Shared {
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[kStages], kv_empty[kStages];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint32_t tmem;
+  int abort;
+  int blocks;
+  int warp_sums[16];
+  Work work[2];
+  int low[kMaxListed + 1], high[kMaxListed + 1];
+};
+constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + kStages) * kTile + sizeof(Shared);
+
+struct PrefillArgs {
+  PagedCache c;
+  const bf16* q;
+  const bf16* k;
+  const bf16* v;
+  bf16* out;
+  float* records;  // [grid][2][256][kRecord] where the key tiles are dealt in runs, else null
+  int* lists;      // [2][kMaxListed + 1]: blocks before each sequence, key tiles before each block
+  int tokens;
+  int q_heads;
+};
+
+// K-major operand, 128-byte swizzle: 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// MN-major operand (V: the head's dimensions contiguous): 64-column halves kHalf apart, 8-key groups 1024.
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
+  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kHalf >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16: fp32 D, bf16 A and B, M = N = 128; B transposed (MN-major) when transpose_b.
+__device__ __forceinline__ constexpr uint32_t instr_desc(bool transpose_b) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (transpose_b ? (1u << 16) : 0u) | (static_cast<uint32_t>(kBN >> 3) << 17) |
+         (static_cast<uint32_t>(kBM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::
+          "r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// 32 consecutive 32-bit columns of this warp's 32 TMEM lanes (one row per lane); no wait.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// The wait for this thread's loads; the loaded registers pass through it, so no use of them moves ahead.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A row key by key, by a whole warp: o (4 dimensions per lane), maximum and sum over keys [from, to).
+__device__ __noinline__ void attend_row(const PagedCache& c, const bf16* q_row, const bf16* k, const bf16* v, int s,
+                                        int kv_head, int from, int to, float* o, float* top, float* sum) {
+  const int lane = threadIdx.x & 31;
+  const uint2 raw = *reinterpret_cast<const uint2*>(q_row + lane * 4);
+  const float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
+                      __uint_as_float(raw.y & 0xffff0000u)};
+  float m = -INFINITY, l = 0.f;
+  o[0] = o[1] = o[2] = o[3] = 0.f;
+  for (int key = from; key < to; ++key) {
+    const int64_t at = (c.page_row(c.page(s, key), kv_head) + (key & (c.page_size() - 1))) * 128 + lane * 4;
+    const uint2 kr = *reinterpret_cast<const uint2*>(k + at), vr = *reinterpret_cast<const uint2*>(v + at);
+    float dot = x[0] * __uint_as_float(kr.x << 16) + x[1] * __uint_as_float(kr.x & 0xffff0000u) +
+                x[2] * __uint_as_float(kr.y << 16) + x[3] * __uint_as_float(kr.y & 0xffff0000u);
+    dot = warp_sum(dot);
+    const float next = fmaxf(m, dot), base = next == -INFINITY ? 0.f : next * kScaleLog2;
+    const float keep = exp2_approx(m * kScaleLog2 - base), p = exp2_approx(dot * kScaleLog2 - base);
+    m = next;
+    l = l * keep + p;
+    o[0] = o[0] * keep + p * __uint_as_float(vr.x << 16);
+    o[1] = o[1] * keep + p * __uint_as_float(vr.x & 0xffff0000u);
+    o[2] = o[2] * keep + p * __uint_as_float(vr.y << 16);
+    o[3] = o[3] * keep + p * __uint_as_float(vr.y & 0xffff0000u);
+  }
+  *top = m;
+  *sum = l;
+}
+
+// --------------------------------------------------------------------------- the list of work
+
+// A sequence's new tokens [begin, end) of q's rows, and its length; no tokens where the offsets are none.
+struct Span {
+  int begin, tokens, length;
+};
+__device__ __forceinline__ Span span_of(const PagedCache& c, int s, int rows) {
+  const int b = __ldg(c.cu_tokens + s), e = __ldg(c.cu_tokens + s + 1);
+  if (b < 0 || e < b || e > rows) {
+    report(c.err, kErrPositionRange);
+    return Span{0, 0, 0};
+  }
+  const int length = c.length(s);
+  if (e - b > length) report(c.err, kErrPositionRange);
+  return Span{b, e - b, length};
+}
+
+// The piece of block `b` of sequence `s`: key tiles [tile0, tile1) (tile1 < 0: all of them).
+__device__ __forceinline__ int block_keys(const Span& x, int b, int per_block) {
+  return max(0, x.length - x.tokens + min((b + 1) * per_block, x.tokens));
+}
+__device__ __forceinline__ int tiles_of(int keys) { return max(1, (keys + kBN - 1) / kBN); }
+
+__device__ __forceinline__ Work make_work(const Span& x, int s, int b, int kv_head, int per_tile, int tile0, int tile1) {
+  Work w;
+  w.token0 = x.begin + b * 2 * per_tile;
+  w.tokens = min(2 * per_tile, x.tokens - b * 2 * per_tile);
+  w.position0 = x.length - x.tokens + b * 2 * per_tile;
+  w.sequence = s;
+  w.kv_head = kv_head;
+  w.keys = max(0, w.position0 + w.tokens);
+  w.tile0 = tile0;
+  w.record = -1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int mine = min(per_tile, w.tokens - i * per_tile);  // tokens of this query tile
+    const int tiles = mine > 0 ? tiles_of(w.position0 + i * per_tile + mine) : 0;
+    w.count[i] = max(0, min(tiles, tile1 < 0 ? tiles : tile1) - tile0);
+  }
+  return w;
+}
+
+// exclusive prefix sums of x over the block's threads; the total in *total
+__device__ int block_scan(int x, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int scan = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += up;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = scan;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int n = warp_sums[w];
+    if (w < warp) before += n;
+    all += n;
+  }
+  *total = all;
+  return before + scan - x;
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefillArgs a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* s_q = smem;
+  unsigned char* ring = smem + 2 * kTile;
+  Shared& sh = *reinterpret_cast<Shared*>(ring + kStages * kTile);
+  volatile int* abort_flag = &sh.abort;
+  const PagedCache& c = a.c;
+  int* err = c.err;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.q_heads / c.kv_heads;
+  const int per_tile = kBM / group, per_block = 2 * per_tile;  // tokens
+  const bool in_runs = a.records != nullptr;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_empty, 1 + 8);  // the last S of the piece, and every softmax warp's look at the list
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sh.kv_full[s], 1);
+      mbar_init(&sh.kv_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.o_empty[i], 128);
+    }
+    sh.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+
+  // ------------------------------------------------------------------ blocks
+  // In runs: sh.low = blocks before each sequence, sh.high = key tiles before each block. Otherwise
+  // sh.low .. sh.high: the sequence's blocks as numbers that grow with their keys (block 0 of a sequence
+  // on a context starts at the context's length in blocks).
+  int blocks = 0;
+  for (int base = 0; base < c.sequences; base += kThreads) {
+    const int s = base + threadIdx.x;
+    Span x{0, 0, 0};
+    if (s < c.sequences) x = span_of(c, s, a.tokens);
+    const int n = (x.tokens + per_block - 1) / per_block;
+    int all;
+    const int before = block_scan(n, sh.warp_sums, &all);
+    if (s < c.sequences && s < kMaxListed) {
+      const int first = max(0, x.length - x.tokens) / per_block;
+      sh.low[s] = in_runs ? min(blocks + before, kMaxListed) : first;
+      if (!in_runs) sh.high[s] = first + n;
+    }
+    blocks += all;
+  }
+  int tiles = 0;
+  if (in_runs) {
+    blocks = min(blocks, kMaxListed);
+    const int listed = min(c.sequences, kMaxListed);
+    if (threadIdx.x == 0) sh.low[listed] = blocks;
+    __syncthreads();
+    for (int base = 0; base < blocks; base += kThreads) {
+      const int i = base + threadIdx.x;
+      int n = 0;
+      if (i < blocks) {
+        int lo = 0, hi = listed;  // the last sequence with low[s] <= i
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (sh.low[mid] <= i) lo = mid;
+          else hi = mid;
+        }
+        n = tiles_of(block_keys(span_of(c, lo, a.tokens), i - sh.low[lo], per_block));
+      }
+      int all;
+      const int before = block_scan(n, sh.warp_sums, &all);
+      if (i < blocks) sh.high[i] = tiles + before;
+      tiles += all;
+    }
+    if (threadIdx.x == 0) sh.high[blocks] = tiles;
+    __syncthreads();
+    if (blockIdx.x == 0) {
+      for (int i = threadIdx.x; i <= kMaxListed; i += kThreads) {
+        if (i <= listed) a.lists[i] = sh.low[i];
+        if (i <= blocks) a.lists[kMaxListed + 1 + i] = sh.high[i];
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int64_t units = static_cast<int64_t>(tiles) * c.kv_heads;
+  const int runs = static_cast<int>(min(units, static_cast<int64_t>(gridDim.x)));
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------------ work list and loads
+    const int ps = c.page_size(), subs = kBN >> c.page_shift;
+    const int64_t works = static_cast<int64_t>(blocks) * c.kv_heads;
+    int64_t unit = 0, unit_end = 0;  // in runs
+    if (in_runs && static_cast<int>(blockIdx.x) < runs) {
+      unit = units * blockIdx.x / runs;
+      unit_end = units * (blockIdx.x + 1) / runs;
+    }
+    const bool listed = c.sequences <= kMaxListed;
+    auto range_of = [&](int s, int* low, int* high) {
+      if (listed) {
+        *low = sh.low[s];
+        *high = sh.high[s];
+      } else {
+        const Span x = span_of(c, s, a.tokens);
+        *low = max(0, x.length - x.tokens) / per_block;
+        *high = *low + (x.tokens + per_block - 1) / per_block;
+      }
+    };
+    // the `rank`-th block in descending order of its number; the whole warp takes part
+    auto select = [&](int rank, int* seq, int* block) {
+      auto at_least = [&](int x) {
+        int n = 0;
+        for (int s = lane; s < c.sequences; s += 32) {
+          int low, high;
+          range_of(s, &low, &high);
+          n += max(0, high - max(low, x));
+        }
+        return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+      };
+      int most = 0;
+      for (int s = lane; s < c.sequences; s += 32) {
+        int low, high;
+        range_of(s, &low, &high);
+        most = max(most, high);
+      }
+      int lo = 0, hi = static_cast<int>(__reduce_max_sync(0xffffffffu, most));  // at_least(lo) > rank >= at_least(hi)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (at_least(mid) > rank) lo = mid;
+        else hi = mid;
+      }
+      int left = rank - at_least(lo + 1);  // so many sequences with a block `lo` come before
+      for (int base = 0; base < c.sequences; base += 32) {
+        const int s = base + lane;
+        int low = 0, high = 0;
+        if (s < c.sequences) range_of(s, &low, &high);
+        const unsigned has = __ballot_sync(0xffffffffu, s < c.sequences && low <= lo && lo < high);
+        const int n = __popc(has);
+        if (left < n) {
+          const int at = __fns(has, 0, left + 1);
+          *seq = base + at;
+          *block = lo - __shfl_sync(0xffffffffu, low, at);
+          return;
+        }
+        left -= n;
+      }
+      *seq = 0;
+      *block = 0;
+    };
+
+    int slot = 0, piece = 0;
+    uint32_t phase = 0, armed = 0;  // bit s: parity armed on kv_full[s]; bit 16 + s: armed at all
+    bool ok = true;
+    for (int64_t round = 0; ok && !*abort_flag; ++round, ++piece) {
+      Work w;
+      if (in_runs) {
+        if (unit >= unit_end) break;
+        int lo = 0, hi = blocks;  // the block of this unit: the last with high[i] * kv_heads <= unit
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (static_cast<int64_t>(sh.high[mid]) * c.kv_heads <= unit) lo = mid;
+          else hi = mid;
+        }
+        const int block = lo, n = sh.high[block + 1] - sh.high[block];
+        const int r = static_cast<int>(unit - static_cast<int64_t>(sh.high[block]) * c.kv_heads);
+        const int tile0 = r % n, tile1 = static_cast<int>(min(static_cast<int64_t>(n), tile0 + unit_end - unit));
+        lo = 0;
+        hi = min(c.sequences, kMaxListed);
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (sh.low[mid] <= block) lo = mid;
+          else hi = mid;
+        }
+        w = make_work(span_of(c, lo, a.tokens), lo, block - sh.low[lo], r / n, per_tile, tile0, tile1);
+        if (tile0 > 0 || tile1 < n) w.record = static_cast<int>(blockIdx.x) * 2 + (round == 0 ? 0 : 1);
+        unit += tile1 - tile0;
+      } else {
+        const int64_t rank = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        if (round * static_cast<int64_t>(gridDim.x) >= works) break;
+        if (rank >= works) {
+          --piece;  // nothing this round; the next one is empty
+          continue;
+        }
+        int s, b;
+        select(static_cast<int>(rank / c.kv_heads), &s, &b);
+        w = make_work(span_of(c, s, a.tokens), s, b, static_cast<int>(rank % c.kv_heads), per_tile, 0, -1);
+      }
+      if (!mbar_wait(&sh.q_empty, (piece & 1) ^ 1, err)) ok = false;
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane == 0) {
+        sh.work[piece & 1] = w;
+        const int rows = group * per_tile * 128;  // bytes of a query tile's half
+        const int n = w.tokens > per_tile ? 2 : 1;
+        mbar_expect_tx(&sh.q_full, 2 * rows * n);
+        for (int i = 0; i < n; ++i) {
+          const uint32_t dst = smem_addr(s_q) + i * kTile;
+          tma_load_3d(dst, &map_q, &sh.q_full, 0, w.kv_head * group, w.token0 + i * per_tile);
+          tma_load_3d(dst + kHalf, &map_q, &sh.q_full, 64, w.kv_head * group, w.token0 + i * per_tile);
+        }
+      }
+      const int steps = max(w.count[0], w.count[1]);
+      auto page_row = [&](int step) {  // this lane's part of the tile, -1 for none
+        const int key = (w.tile0 + step) * kBN + lane * ps;
+        if (lane >= subs || step >= steps || key >= w.keys) return -1;
+        return static_cast<int>(c.page_row(c.page(w.sequence, key), w.kv_head));
+      };
+      int row = page_row(0);
+      for (int step = 0; ok && step < steps; ++step) {
+        const int next = page_row(step + 1);
+        const int parts = __popc(__ballot_sync(0xffffffffu, row >= 0));
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!mbar_wait(&sh.kv_empty[slot], phase ^ 1, err)) ok = false;
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(&sh.kv_full[slot], parts * ps * 256);
+          __syncwarp();
+          if (row >= 0) {
+            const CUtensorMap* map = kv ? &map_v : &map_k;
+            const uint32_t dst = smem_addr(ring) + slot * kTile + lane * ps * 128;
+            tma_load_2d(dst, map, &sh.kv_full[slot], 0, row);
+            tma_load_2d(dst + kHalf, map, &sh.kv_full[slot], 64, row);
+          }
+          armed = (armed & ~(1u << slot)) | (phase << slot) | (1u << (16 + slot));
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+        row = next;
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    // tell the others that the list has ended
+    if (ok && !*abort_flag && mbar_wait(&sh.q_empty, (piece & 1) ^ 1, err)) {
+      __syncwarp();
+      if (lane == 0) {
+        sh.work[piece & 1].token0 = -1;
+        mbar_arrive(&sh.q_full);
+      }
+    } else {
+      *abort_flag = 1;
+    }
+    // copies and arrivals in flight land before the CTA's shared memory goes away
+    for (int s = 0; s < kStages; ++s) {
+      if (!(armed & (1u << (16 + s)))) continue;
+      mbar_wait(&sh.kv_full[s], (armed >> s) & 1u, err);
+      if (!*abort_flag) mbar_wait(&sh.kv_empty[s], (armed >> s) & 1u, err);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------------ MMA issue
+    const uint32_t idesc_s = instr_desc(false), idesc_o = instr_desc(true);
+    int it = 0;  // K and V tiles taken so far
+    uint32_t p_seen[2] = {0, 0}, o_seen[2] = {0, 0};
+    bool ok = true;
+    for (int piece = 0; ok && !*abort_flag; ++piece) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh.q_full, piece & 1, err))) {
+        ok = false;
+        break;
+      }
+      const Work w = sh.work[piece & 1];
+      if (w.token0 < 0) break;
+      tc_fence_after();
+      const int steps = max(w.count[0], w.count[1]);
+      auto wait_tile = [&](int index) {
+        return __all_sync(0xffffffffu, mbar_wait(&sh.kv_full[index % kStages], (index / kStages) & 1, err));
+      };
+      auto issue_s = [&](int i, int index) {  // S_i = Q_i K^T
+        const uint32_t qa = smem_addr(s_q) + i * kTile, ka = smem_addr(ring) + (index % kStages) * kTile;
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kHalf;
+          mma_smem(tmem + i * kBN, desc_kmajor(qa + off) + 2 * (kk & 3), desc_kmajor(ka + off) + 2 * (kk & 3), idesc_s,
+                   kk > 0 ? 1u : 0u);
+        }
+        mma_commit(&sh.s_full[i]);
+      };
+      auto issue_o = [&](int i, int index, bool first) {  // O_i (+)= P_i V
+        const uint32_t va = smem_addr(ring) + (index % kStages) * kTile;
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk)
+          mma_tmem(tmem + 256 + i * kBN, tmem + i * kBN + kk * 8, desc_mnmajor(va + kk * 16 * 128), idesc_o,
+                   (!first || kk > 0) ? 1u : 0u);
+      };
+      if (!wait_tile(it)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        for (int i = 0; i < 2; ++i)
+          if (w.count[i] > 0) issue_s(i, it);
+        mma_commit(&sh.kv_empty[it % kStages]);
+        if (steps == 1) mma_commit(&sh.q_empty);
+      }
+      __syncwarp();
+      for (int step = 0; step < steps && ok; ++step) {
+        const int v_index = it + 2 * step + 1, k_index = it + 2 * step + 2;
+        if (!wait_tile(v_index)) {
+          ok = false;
+          break;
+        }
+        const int valid = w.keys - (w.tile0 + step) * kBN;
+        if (valid < kBN) {  // values past the block's keys: zeros, whatever is there
+          const uint32_t va = smem_addr(ring) + (v_index % kStages) * kTile;
+          for (int r = max(valid, 0) + (lane >> 3); r < kBN; r += 4)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(va + h * kHalf + r * 128 + (lane & 7) * 16), "r"(0)
+                           : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        for (int i = 0; i < 2 && ok; ++i) {
+          if (step < w.count[i]) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh.p_full[i], p_seen[i] & 1, err)) ||
+                (step == 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.o_empty[i], (o_seen[i] & 1) ^ 1, err)))) {
+              ok = false;
+              break;
+            }
+            ++p_seen[i];
+            tc_fence_after();
+            if (lane == 0) {
+              issue_o(i, v_index, step == 0);
+              if (step + 1 == w.count[i]) mma_commit(&sh.o_full[i]);
+            }
+            __syncwarp();
+          }
+          // The next scores overwrite this tile's P: one thread's MMAs run in the order of their issue.
+          if (step + 1 < w.count[i]) {
+            if (i == 0 || w.count[0] <= step + 1) {
+              if (!wait_tile(k_index)) {
+                ok = false;
+                break;
+              }
+            }
+            tc_fence_after();
+            if (lane == 0) issue_s(i, k_index);
+            __syncwarp();
+          }
+        }
+        if (ok && lane == 0) {
+          mma_commit(&sh.kv_empty[v_index % kStages]);
+          if (step + 1 < steps) mma_commit(&sh.kv_empty[k_index % kStages]);
+          if (step + 2 == steps) mma_commit(&sh.q_empty);
+        }
+        __syncwarp();
+      }
+      it += 2 * steps;
+      for (int i = 0; i < 2; ++i)
+        if (w.count[i] > 0) ++o_seen[i];
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    // ------------------------------------------------------------------ softmax, one row per thread
+    const int i = warp >> 2;                                  // query tile
+    const int r = (warp & 3) * 32 + lane;                     // row of it
+    const int place = r / group, head = r - place * group;    // token and query head of the row
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + i * kBN, t_o = tmem + lanes + 256 + i * kBN;
+    uint32_t s_seen = 0, o_seen = 0;
+    bool ok = true;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)); };
+    for (int piece = 0; ok && !*abort_flag; ++piece) {
+      if (!wait_all(&sh.q_full, piece & 1)) {
+        ok = false;
+        break;
+      }
+      const Work w = sh.work[piece & 1];
+      if (w.token0 < 0) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_empty);
+      const int count = w.count[i];
+      const int token = i * per_tile + place;
+      const bool real = place < per_tile && token < w.tokens;
+      const int limit = real ? max(0, w.position0 + token + 1) : 0;  // keys the row sees
+      float m = -INFINITY, l = 0.f;
+      for (int step = 0; step < count && ok; ++step) {
+        if (!wait_all(&sh.s_full[i], s_seen & 1)) {
+          ok = false;
+          break;
+        }
+        ++s_seen;
+        tc_fence_after();
+        uint32_t x[kBN];
+#pragma unroll
+        for (int b = 0; b < kBN / 32; ++b) tmem_ld32(t_s + b * 32, x + b * 32);
+#pragma unroll
+        for (int b = 0; b < kBN / 32; ++b) tmem_ld_wait(x + b * 32);
+        const int seen = limit - (w.tile0 + step) * kBN;  // of this tile's keys
+        if (__any_sync(0xffffffffu, seen < kBN)) {
+#pragma unroll
+          for (int e = 0; e < kBN; ++e)
+            if (e >= seen) x[e] = __float_as_uint(-INFINITY);
+        }
+        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < kBN; ++e) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(x[e]));
+        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+        const bool moves = top > m + kSlack || (m == -INFINITY && top > m);
+        const float next = moves ? top : m;
+        const float base = next == -INFINITY ? 0.f : next * kScaleLog2;
+        if (step > 0 && __any_sync(0xffffffffu, moves)) {  // the products of the tile before have finished: S came after
+          const float keep = exp2_approx(m * kScaleLog2 - base);
+          l *= moves ? keep : 1.f;
+#pragma unroll
+          for (int b = 0; b < kD / 32; ++b) {
+            uint32_t o[32];
+            tmem_ld32(t_o + b * 32, o);
+            tmem_ld_wait(o);
+            if (moves) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            }
+            tmem_st32(t_o + b * 32, o);
+          }
+        }
+        m = next;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float p0 = exp2_approx(__uint_as_float(x[b * 64 + 2 * e]) * kScaleLog2 - base);
+            const float p1 = exp2_approx(__uint_as_float(x[b * 64 + 2 * e + 1]) * kScaleLog2 - base);
+            sum[(2 * e) & 3] += p0;
+            sum[(2 * e + 1) & 3] += p1;
+            packed[e] = pack_bf16x2(p0, p1);
+          }
+          tmem_st32(t_s + b * 32, packed);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        mbar_arrive(&sh.p_full[i]);
+      }
+      if (!ok) break;
+      if (count > 0 && !wait_all(&sh.o_full[i], o_seen & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int64_t out_row = static_cast<int64_t>(w.token0 + token) * a.q_heads + w.kv_head * group + head;
+      float* rec = w.record < 0 ? nullptr : a.records + (static_cast<int64_t>(w.record) * 2 * kBM + i * kBM + r) * kRecord;
+      const float inv = limit > 0 ? 1.f / l : 0.f;
+      bool finite = true;
+      if (count > 0) {
+#pragma unroll
+        for (int b = 0; b < kD / 32; ++b) {
+          uint32_t o[32];
+          tmem_ld32(t_o + b * 32, o);
+          tmem_ld_wait(o);
+          if (!real) continue;
+          float f[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            f[e] = l > 0.f || l != l ? __uint_as_float(o[e]) * (rec ? 1.f : inv) : 0.f;
+            finite = finite && fabsf(f[e]) <= 3.4e38f;
+          }
+          if (rec) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              *reinterpret_cast<float4*>(rec + b * 32 + 4 * e) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(a.out + out_row * 128 + b * 32 + 8 * e) = pack8(f + 8 * e);
+          }
+        }
+        tc_fence_before();
+        mbar_arrive(&sh.o_empty[i]);
+        ++o_seen;
+      } else if (rec && real) {
+        for (int e = 0; e < kD; e += 4) *reinterpret_cast<float4*>(rec + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      if (rec && real) {
+        rec[128] = m;
+        rec[129] = l;
+      }
+      // rows with something not finite: again, key by key
+      unsigned again = __ballot_sync(0xffffffffu, real && limit > w.tile0 * kBN && count > 0 && !(finite && l > 0.f));
+      __syncwarp();
+      while (again) {
+        const int from = __ffs(again) - 1;
+        again &= again - 1;
+        const int64_t row = __shfl_sync(0xffffffffu, out_row, from);
+        const int keys = __shfl_sync(0xffffffffu, limit, from), first = w.tile0 * kBN;
+        float o[4], top, sum;
+        attend_row(c, a.q + row * 128, a.k, a.v, w.sequence, w.kv_head, first, min(keys, first + count * kBN), o, &top, &sum);
+        if (rec) {
+          float* at = rec + (from - lane) * kRecord;
+          *reinterpret_cast<float4*>(at + lane * 4) = make_float4(o[0], o[1], o[2], o[3]);
+          if (lane == 0) {
+            at[128] = top;
+            at[129] = sum;
+          }
+        } else {
+          const float s = 1.f / sum;
+          *reinterpret_cast<uint2*>(a.out + row * 128 + lane * 4) =
+              make_uint2(pack_bf16x2(o[0] * s, o[1] * s), pack_bf16x2(o[2] * s, o[3] * s));
+        }
+      }
+    }
+    if (!ok) *abort_flag = 1;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+// One warp per (token, query head) whose block's key tiles lie in more than one run: merges the records.
+__global__ void __launch_bounds__(128) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
+  pdl_wait();
+  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x) >> 5;
+  const PagedCache& c = a.c;
+  if (warp >= static_cast<int64_t>(a.tokens) * a.q_heads) return;
+  const int lane = threadIdx.x & 31;
+  const int t = static_cast<int>(warp / a.q_heads), head = static_cast<int>(warp % a.q_heads);
+  const int s = find_sequence(c.cu_tokens, c.sequences, t);
+  if (s < 0) return;
+  const Span x = span_of(c, s, a.tokens);
+  if (t < x.begin || t >= x.begin + x.tokens || s >= kMaxListed) return;
+  const int group = a.q_heads / c.kv_heads, per_tile = kBM / group, per_block = 2 * per_tile;
+  const int listed = min(c.sequences, kMaxListed);
+  const int blocks = __ldcg(a.lists + listed);
+  const int place = t - x.begin, block = __ldcg(a.lists + s) + place / per_block;
+  if (block >= blocks) return;
+  const int* before = a.lists + kMaxListed + 1;
+  const int tile0 = __ldcg(before + block), n = __ldcg(before + block + 1) - tile0;
+  const int64_t units = static_cast<int64_t>(__ldcg(before + blocks)) * c.kv_heads;
+  const int runs = static_cast<int>(min(units, static_cast<int64_t>(ctas)));
+  const int64_t first = static_cast<int64_t>(tile0) * c.kv_heads + static_cast<int64_t>(head / group) * n;
+  const int run_lo = static_cast<int>(((first + 1) * runs - 1) / units);
+  const int run_hi = static_cast<int>(((first + n) * runs - 1) / units);
+  if (run_lo == run_hi) return;  // whole, already written
+  const int slot_lo = units * run_lo / runs == first ? 0 : 1;
+  const int in_block = place % per_block, tile = in_block / per_tile;
+  const int r = tile * kBM + (in_block - tile * per_tile) * group + head % group;
+  auto record = [&](int run) {
+    return a.records + ((static_cast<int64_t>(run) * 2 + (run == run_lo ? slot_lo : 0)) * 2 * kBM + r) * kRecord;
+  };
+  float top = -INFINITY;
+  for (int run = run_lo + lane; run <= run_hi; run += 32) top = fmaxf(top, __ldcg(record(run) + 128));
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int run = run_lo; run <= run_hi; ++run) {
+    const float* rec = record(run);
+    const float4 y = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
+    const float e = exp2_approx(__ldcg(rec + 128) * kScaleLog2 - base);
+    sum += e * __ldcg(rec + 129);
+    o.x += e * y.x;
+    o.y += e * y.y;
+    o.z += e * y.z;
+    o.w += e * y.w;
+  }
+  const float inv = x.length - x.tokens + place >= 0 ? 1.f / sum : 0.f;  // no position: no keys
+  const bool none = inv == 0.f && x.length - x.tokens + place < 0;
+  *reinterpret_cast<uint2*>(a.out + warp * 128 + lane * 4) =
+      none ? make_uint2(0u, 0u) : make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+}
+
+constexpr size_t kListBytes = (2 * (kMaxListed + 1) * sizeof(int) + 255) / 256 * 256;
+
+// most blocks that `tokens` new tokens of `sequences` sequences make
+int64_t most_blocks(int64_t tokens, int sequences, int group) {
+  const int64_t per_block = 2 * (kBM / group);
+  return std::min<int64_t>((tokens + sequences * (per_block - 1)) / per_block, tokens);
+}
+
+// Whether the key tiles are dealt in runs: where whole blocks would leave SMs idle for long.
+bool deal_in_runs(int64_t tokens, int sequences, int q_heads, int kv_heads) {
+  const int64_t blocks = most_blocks(tokens, sequences, q_heads / kv_heads);
+  return blocks <= kMaxListed && sequences <= kMaxListed && blocks * kv_heads < 2 * sm_count();
+}
+
+}  // namespace
+
+size_t paged_prefill_workspace_bytes(int64_t tokens, int sequences, int q_heads, int kv_heads) {
+  if (!deal_in_runs(tokens, sequences, q_heads, kv_heads)) return 0;
+  return kListBytes + static_cast<size_t>(sm_count()) * 2 * 2 * kBM * kRecord * sizeof(float);
+}
+
+cudaError_t launch_paged_prefill(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
+                                 int64_t tokens, int q_heads, void* workspace, cudaStream_t stream) {
+  const int group = q_heads / c.kv_heads, page_size = 1 << c.page_shift;
+  const int rows = static_cast<int>(static_cast<int64_t>(c.num_pages) * c.kv_heads * page_size);
+  CUtensorMap mq, mk, mv;
+  if (!make_map_3d(&mq, q, kD, q_heads, static_cast<int>(tokens), q_heads, group, 64, kBM / group) ||
+      !make_map_2d(&mk, k_pages, rows, kD, page_size, 64) || !make_map_2d(&mv, v_pages, rows, kD, page_size, 64))
+    return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(kSmem));
+  if (e != cudaSuccess) return e;
+  PrefillArgs a{};
+  a.c = c;
+  a.q = static_cast<const bf16*>(q);
+  a.k = static_cast<const bf16*>(k_pages);
+  a.v = static_cast<const bf16*>(v_pages);
+  a.out = static_cast<bf16*>(out);
+  a.tokens = static_cast<int>(tokens);
+  a.q_heads = q_heads;
+  const bool in_runs = deal_in_runs(tokens, c.sequences, q_heads, c.kv_heads);
+  int64_t grid = most_blocks(tokens, c.sequences, group) * c.kv_heads;
+  if (in_runs) {
+    a.lists = static_cast<int*>(workspace);
+    a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kListBytes);
+    grid *= std::max<int64_t>(1, ((static_cast<int64_t>(c.max_pages) << c.page_shift) + kBN - 1) / kBN);
+  }
+  grid = std::min<int64_t>(grid, sm_count());
+  paged_prefill_kernel<<<static_cast<unsigned>(grid), kThreads, kSmem, stream>>>(mq, mk, mv, a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !in_runs) return e;
+  const int64_t warps = tokens * q_heads;
+  return launch_pdl(paged_prefill_merge_kernel, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, stream, a,
+                    static_cast<int>(grid));
+}
+
+}  // namespace ipe

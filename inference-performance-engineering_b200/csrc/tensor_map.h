@@ -13,9 +13,9 @@ bool make_map_2d(CUtensorMap* map, const void* ptr, int rows, int k, int box_row
 
 // Slices of a K-contiguous bf16 array: `slices` matrices of `rows` rows (of k elements), slice s
 // starting slice_rows * s rows in; rows >= `rows` of a slice read as zeros (TMA out-of-bounds fill),
-// so a slice can stop short of its allocation. Boxes of box_k x box_rows x 1, 128-byte swizzle.
+// so a slice can stop short of its allocation. Boxes of box_k x box_rows x box_slices, 128-byte swizzle.
 bool make_map_3d(CUtensorMap* map, const void* ptr, int k, int rows, int slices, int64_t slice_rows, int box_rows,
-                 int box_k);
+                 int box_k, int box_slices = 1);
 
 int sm_count();
 

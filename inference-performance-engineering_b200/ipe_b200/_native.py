@@ -52,7 +52,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                            c_size_t, _P]),
     "ipe_paged_decode_attention_workspace": (c_size_t, [c_int, c_int, c_int]),
     "ipe_paged_prefill_attention": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int64, c_int,
-                                            c_int, _P]),
+                                            c_int, _P, c_size_t, _P]),
+    "ipe_paged_prefill_attention_workspace": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "ipe_shared_prefix_attention": (c_int, [_P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int,
                                             c_int, _P]),
     "ipe_gemm": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P]),

@@ -147,9 +147,10 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if cu_tokens.shape != (sequences + 1,):
         raise ValueError(f"{name}: cu_tokens must be [sequences + 1]")
     with _on(device):
+        ws = _workspace(device, "ipe_paged_prefill_attention_workspace", q.shape[0], sequences, q_heads, kv_heads)
         nat.call("ipe_paged_prefill_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                  page_table.data_ptr(), cu_tokens.data_ptr(), lengths.data_ptr(), out.data_ptr(), q.shape[0], sequences,
-                 q_heads, kv_heads, pages, page_size, width, _stream(device))
+                 q_heads, kv_heads, pages, page_size, width, ws.data_ptr(), ws.numel(), _stream(device))
     return out
 
 
