@@ -287,7 +287,9 @@ size_t ipe_paged_prefill_attention_workspace(int64_t tokens, int sequences, int 
 int ipe_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* prefix_pages,
                                 int prefix_count, const int32_t* page_table, const int32_t* lengths, void* out,
                                 int sequences, int q_heads, int kv_heads, int64_t num_pages, int page_size,
-                                int max_pages, void* stream);
+                                int max_pages, void* workspace, size_t workspace_bytes, void* stream);
+size_t ipe_shared_prefix_attention_workspace(int sequences, int q_heads, int kv_heads, int page_size,
+                                             int prefix_count);
 
 /* ------------------------------------------------------------------ tensor-core GEMM */
 

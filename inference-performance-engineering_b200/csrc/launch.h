@@ -92,8 +92,9 @@ void launch_qk_norm_rope_append_f32(const void* qkv, int batch, int tokens, int 
 cudaError_t launch_attention_f32(const void* q, const void* k, const void* v, void* out, int batch, int q_heads,
                                  int kv_heads, int tokens, int capacity, int start, cudaStream_t stream);
 
-// Paged cache (paged_append.cu, paged_decode.cu, paged_prefill.cu, paged_attention.cu); PagedCache is in paged.cuh.
+// Paged cache (paged_append.cu, paged_decode.cu, paged_prefill.cu); PagedCache is in paged.cuh.
 struct PagedCache;
+struct SharedKeys;
 cudaError_t launch_paged_append(const PagedCache& c, const void* qkv, int64_t tokens, int q_heads, const void* q_norm,
                                 const void* k_norm, const void* cos_t, const void* sin_t, bool fp32_tables,
                                 int64_t table_rows, void* q_out, void* k_pages, void* v_pages, float eps,
@@ -104,8 +105,12 @@ cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* 
 size_t paged_prefill_workspace_bytes(int64_t tokens, int sequences, int q_heads, int kv_heads);
 cudaError_t launch_paged_prefill(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
                                  int64_t tokens, int q_heads, void* workspace, cudaStream_t stream);
-cudaError_t launch_paged_attention(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages,
-                                   void* out, int64_t tokens, int q_heads, cudaStream_t stream);
+SharedKeys shared_keys_plan(const PagedCache& c, int q_heads);
+cudaError_t launch_shared_keys(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, int q_heads,
+                               const SharedKeys& plan, cudaStream_t stream);
+size_t shared_prefix_workspace_bytes(const PagedCache& c, int q_heads);
+cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
+                                 int q_heads, void* workspace, cudaStream_t stream);
 
 void launch_add_partial(void* x, const float* sum, int64_t count, cudaStream_t stream);
 

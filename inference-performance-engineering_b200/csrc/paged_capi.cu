@@ -3,7 +3,7 @@
 #include <cstdio>
 
 #include "launch.h"
-#include "paged.cuh"
+#include "paged_records.cuh"
 
 namespace ipe {
 int report_failure(int status, const char* message);
@@ -40,7 +40,7 @@ int paged_cache(const char* name, const void* k_pages, const void* v_pages, cons
                 static_cast<long long>(tokens), sequences, static_cast<long long>(num_pages), max_pages);
   // positions, cache rows and (token, head) rows are 32-bit numbers in the kernels; their byte offsets are 64-bit
   if (tokens * q_heads > INT32_MAX || num_pages > INT32_MAX / (static_cast<int64_t>(kv_heads) * page_size) ||
-      max_pages > (1 << 30) / page_size || sequences > (1 << 24))
+      max_pages > (1 << 27) / page_size || sequences > (1 << 24))
     return fail(IPE_ERR_UNSUPPORTED, "%s: sizes past the kernels' 32-bit row numbers", name);
   if (tokens == 0 || sequences == 0) return IPE_OK;
   if (!k_pages || !v_pages || !page_table || !lengths) return fail(IPE_ERR_ARGUMENT, "%s: null pointer", name);
@@ -83,6 +83,17 @@ size_t ipe_paged_decode_attention_workspace(int sequences, int q_heads, int kv_h
 size_t ipe_paged_prefill_attention_workspace(int64_t tokens, int sequences, int q_heads, int kv_heads) {
   if (tokens < 1 || sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8) return 0;
   return ipe::paged_prefill_workspace_bytes(tokens, sequences, q_heads, kv_heads);
+}
+
+size_t ipe_shared_prefix_attention_workspace(int sequences, int q_heads, int kv_heads, int page_size, int prefix_count) {
+  if (sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8 || page_size < 1 || prefix_count < 0)
+    return 0;
+  ipe::PagedCache c{};
+  c.sequences = sequences;
+  c.kv_heads = kv_heads;
+  c.prefix_count = prefix_count;
+  while ((1 << c.page_shift) < page_size) ++c.page_shift;
+  return ipe::shared_prefix_workspace_bytes(c, q_heads);
 }
 
 int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, int kv_heads,
@@ -152,7 +163,7 @@ int ipe_paged_prefill_attention(const void* q, const void* k_pages, const void* 
 int ipe_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* prefix_pages,
                                 int prefix_count, const int32_t* page_table, const int32_t* lengths, void* out,
                                 int sequences, int q_heads, int kv_heads, int64_t num_pages, int page_size,
-                                int max_pages, void* stream) {
+                                int max_pages, void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "ipe_shared_prefix_attention";
   ipe::PagedCache c;
   if (int status = paged_cache(name, k_pages, v_pages, page_table, lengths, sequences, sequences, q_heads, kv_heads,
@@ -166,8 +177,13 @@ int ipe_shared_prefix_attention(const void* q, const void* k_pages, const void* 
     return fail(IPE_ERR_ARGUMENT, "%s: prefix_pages", name);
   c.prefix_pages = prefix_pages;
   c.prefix_count = prefix_count;
-  return finish(ipe::launch_paged_attention(c, q, k_pages, v_pages, out, sequences, q_heads,
-                                            static_cast<cudaStream_t>(stream)),
+  if (ipe::shared_keys_plan(c, q_heads).units > INT32_MAX)
+    return fail(IPE_ERR_UNSUPPORTED, "%s: %d prefix pages for %d sequences are past the kernels' 32-bit numbers", name,
+                prefix_count, sequences);
+  const size_t need = ipe::shared_prefix_workspace_bytes(c, q_heads);
+  if (int status = workspace_checks(name, workspace, workspace_bytes, need)) return status;
+  return finish(ipe::launch_shared_prefix(c, q, k_pages, v_pages, out, q_heads, workspace,
+                                          static_cast<cudaStream_t>(stream)),
                 name);
 }
 

@@ -16,7 +16,7 @@
 #include <algorithm>
 
 #include "launch.h"
-#include "paged.cuh"
+#include "paged_records.cuh"
 #include "tensor_map.h"
 
 namespace ipe {
@@ -30,8 +30,6 @@ constexpr int kStageBytes = 2 * 16 * 256;  // one warp's keys and values of a un
 constexpr int kCtasPerSm = 2;
 constexpr int kHeads = 8;                // columns of the products
 constexpr int kMergeStride = 132;        // floats; spreads a warp's 4 head pairs over the banks
-constexpr int kRecord = 132;             // floats: o[128], maximum, sum, 2 unused
-constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // 128^-0.5 * log2(e)
 constexpr size_t kSmem = static_cast<size_t>(kStages) * kWarps * kStageBytes +
                          static_cast<size_t>(kWarps) * kHeads * kMergeStride * sizeof(float);
 
@@ -43,14 +41,10 @@ struct DecodeArgs {
   bf16* out;
   float* records;    // [grid][2][G][kRecord]
   int64_t* offsets;  // [sequences + 1]: units of one KV head before each sequence
+  float* whole;      // null, or where rows that are not in parts go: [sequences][q_heads][kRecord], not to out
+  int first;         // keys before this one are left out
   int q_heads;
 };
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -58,24 +52,22 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-__device__ __forceinline__ int units_of(const PagedCache& c, int s) { return (c.length(s) + kUnit - 1) / kUnit; }
-
-// The units are dealt to `runs` CTAs, none of them without one; run r begins with unit run_start(r).
-__device__ __forceinline__ int runs_of(int64_t units, int ctas) { return units < ctas ? static_cast<int>(units) : ctas; }
-__device__ __forceinline__ int64_t run_start(int64_t units, int run, int runs) { return units * run / max(runs, 1); }
+// a sequence's keys behind the shared ones
+__device__ __forceinline__ int keys_of(const DecodeArgs& a, int s) { return max(0, a.c.length(s) - a.first); }
+__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
 
 // A place in the batch's sequence of units.
 struct Cursor {
-  int s, h, unit, units, length;
-  __device__ __forceinline__ void advance(const PagedCache& c) {
+  int s, h, unit, units, keys;
+  __device__ __forceinline__ void advance(const DecodeArgs& a) {
     if (++unit < units) return;
     unit = 0;
-    if (++h < c.kv_heads) return;
+    if (++h < a.c.kv_heads) return;
     h = 0;
     do {
       ++s;
-      length = s < c.sequences ? c.length(s) : kUnit;
-      units = (length + kUnit - 1) / kUnit;
+      keys = s < a.c.sequences ? keys_of(a, s) : kUnit;
+      units = units_of(keys);
     } while (units == 0);
   }
 };
@@ -95,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const int per = (c.sequences + kThreads - 1) / kThreads;
   const int s_lo = min(c.sequences, static_cast<int>(threadIdx.x) * per), s_hi = min(c.sequences, s_lo + per);
   int64_t mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) mine += units_of(c, s);
+  for (int s = s_lo; s < s_hi; ++s) mine += units_of(keys_of(a, s));
   int64_t scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -114,13 +106,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const int runs = runs_of(units, gridDim.x);
   const int64_t u0 = run_start(units, blockIdx.x, runs), u1 = run_start(units, blockIdx.x + 1, runs);
   for (int s = s_lo; s < s_hi; ++s) {
-    const int n = units_of(c, s);
+    const int keys = keys_of(a, s), n = units_of(keys);
     if (blockIdx.x == 0) a.offsets[s] = before;
     if (n > 0 && u0 >= before * c.kv_heads && u0 < (before + n) * c.kv_heads) {
       const int r = static_cast<int>(u0 - before * c.kv_heads);
-      start = Cursor{s, r / n, r % n, n, c.length(s)};
+      start = Cursor{s, r / n, r % n, n, keys};
     }
-    if (n == 0 && s % gridDim.x == blockIdx.x) {  // no keys: zeros
+    if (n == 0 && !a.whole && s % gridDim.x == blockIdx.x) {  // no keys: zeros
       uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(s) * a.q_heads * 128);
       for (int i = 0; i < a.q_heads * 16; ++i) row[i] = make_uint4(0, 0, 0, 0);
     }
@@ -128,7 +120,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[c.sequences] = total;
   __syncthreads();
-  if (blockIdx.x >= runs) return;
+  if (blockIdx.x >= runs) {
+    if (a.whole) pdl_wait();
+    return;
+  }
   const int64_t count = u1 - u0;
 
   // ------------------------------------------------------------------ loads
@@ -138,12 +133,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   int page = 0;  // of `ahead`
   auto look_up = [&] {
     const int key0 = ahead.unit * kUnit + warp * 16;
-    page = key0 < ahead.length ? c.page(ahead.s, key0) : 0;
+    page = key0 < ahead.keys ? c.page(ahead.s, a.first + key0) : 0;
   };
   auto issue = [&](int stage) {
     if (issued < count) {
       const int key0 = ahead.unit * kUnit + warp * 16;
-      const int valid = ahead.length - key0;  // keys of these 16 that exist
+      const int valid = ahead.keys - key0;  // keys of these 16 that exist
       const int64_t row0 = c.page_row(page, ahead.h) + (key0 & (c.page_size() - 1));
       const int chunk = lane & 15;
       const uint32_t dst = ring + stage * (kWarps * kStageBytes);
@@ -158,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         cp_async16(dst + 4096 + at, real ? vs + row * 128 : a.v, real ? 16 : 0);
       }
       if (++issued < count) {
-        ahead.advance(c);
+        ahead.advance(a);
         look_up();
       }
     }
@@ -209,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     const int key = at.unit * kUnit + warp * 16 + (lane >> 2);
     float s4[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s4[i] = key + (i >> 1) * 8 < at.length ? sc[0][i] + sc[1][i] : -INFINITY;
+    for (int i = 0; i < 4; ++i) s4[i] = key + (i >> 1) * 8 < at.keys ? sc[0][i] + sc[1][i] : -INFINITY;
     float keep[2], p[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -272,10 +267,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           sum += e * stats[w][g][1];
           o += e * merge[(w * kHeads + g) * kMergeStride + threadIdx.x];
         }
-        if (whole) {
-          a.out[(static_cast<int64_t>(at.s) * a.q_heads + at.h * group + g) * 128 + threadIdx.x] = __float2bfloat16_rn(o / sum);
+        const int64_t row = static_cast<int64_t>(at.s) * a.q_heads + at.h * group + g;
+        if (whole && !a.whole) {
+          a.out[row * 128 + threadIdx.x] = __float2bfloat16_rn(o / sum);
         } else {
-          float* rec = a.records + ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * group + g) * kRecord;
+          float* rec = whole ? a.whole + row * kRecord
+                             : a.records + ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * group + g) * kRecord;
           rec[threadIdx.x] = o;
           if (threadIdx.x == 0) {
             rec[128] = top;
@@ -286,55 +283,88 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       __syncthreads();
       fresh = true;
     }
-    if (u + 1 < count) at.advance(c);
+    if (u + 1 < count) at.advance(a);
   }
+  // beside the kernel of the shared keys: whoever waits for this grid then waits for that one too
+  if (a.whole) pdl_wait();
 }
 
-// One warp per (sequence, query head) whose units lie in more than one run: merges the runs' records.
+// The parts of a row, none where the sequence has no keys or the row is whole.
+__device__ __forceinline__ Parts decode_parts(const DecodeArgs& a, int ctas, int s, int head) {
+  const PagedCache& c = a.c;
+  const int group = a.q_heads / c.kv_heads;
+  Parts p;
+  p.none();
+  const int64_t from = __ldcg(a.offsets + s), n = __ldcg(a.offsets + s + 1) - from;
+  if (n == 0) return p;
+  p.base = a.records;
+  p.rows = group;
+  p.row = head % group;
+  p.find(from * c.kv_heads + head / group * n, n, __ldcg(a.offsets + c.sequences) * c.kv_heads, ctas);
+  if (p.lo == p.hi) {
+    if (a.whole) p.single(a.whole + (static_cast<int64_t>(s) * a.q_heads + head) * kRecord);
+    else p.none();
+  }
+  return p;
+}
+
+// One warp per (sequence, query head) in parts.
 __global__ void __launch_bounds__(kThreads) paged_decode_merge_kernel(const DecodeArgs a, int ctas) {
   pdl_wait();
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  const PagedCache& c = a.c;
-  if (warp >= static_cast<int64_t>(c.sequences) * a.q_heads) return;
-  const int lane = threadIdx.x & 31;
-  const int s = static_cast<int>(warp / a.q_heads), head = static_cast<int>(warp % a.q_heads);
-  const int group = a.q_heads / c.kv_heads, h = head / group, g = head % group;
-  const int64_t from = __ldcg(a.offsets + s), n = __ldcg(a.offsets + s + 1) - from;
-  const int64_t units = __ldcg(a.offsets + c.sequences) * c.kv_heads;
-  if (n == 0) return;  // zeros, already written
-  const int runs = runs_of(units, ctas);
-  const int64_t first = from * c.kv_heads + h * n;  // the item's units: first .. first + n - 1
-  const int run_lo = static_cast<int>(((first + 1) * runs - 1) / units);
-  const int run_hi = static_cast<int>(((first + n) * runs - 1) / units);
-  if (run_lo == run_hi) return;  // whole, already written
-  // a run's first piece is its slot 0: that of every run after the first, and of the first if it begins with the item
-  const int slot_lo = run_start(units, run_lo, runs) == first ? 0 : 1;
-  auto record = [&](int run) {
-    return a.records + ((static_cast<int64_t>(run) * 2 + (run == run_lo ? slot_lo : 0)) * group + g) * kRecord;
-  };
-  float top = -INFINITY;
-  for (int r = run_lo + lane; r <= run_hi; r += 32) top = fmaxf(top, __ldcg(record(r) + 128));
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
-  float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int r = run_lo; r <= run_hi; ++r) {
-    const float* rec = record(r);
-    const float4 x = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
-    const float e = exp2_approx(__ldcg(rec + 128) * kScaleLog2 - base);
-    sum += e * __ldcg(rec + 129);
-    o.x += e * x.x;
-    o.y += e * x.y;
-    o.z += e * x.z;
-    o.w += e * x.w;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  if (row >= static_cast<int64_t>(a.c.sequences) * a.q_heads) return;
+  const Parts parts[1] = {decode_parts(a, ctas, static_cast<int>(row / a.q_heads), static_cast<int>(row % a.q_heads))};
+  if (parts[0].hi >= parts[0].lo) join_parts(parts, a.out + row * 128);
+}
+
+// One warp per (sequence, query head): the parts of the shared keys and those of the sequence's own.
+__global__ void __launch_bounds__(kThreads) shared_prefix_merge_kernel(const DecodeArgs a, int ctas, const SharedKeys shared) {
+  pdl_wait();
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
+  if (row >= static_cast<int64_t>(a.c.sequences) * a.q_heads) return;
+  const int s = static_cast<int>(row / a.q_heads), head = static_cast<int>(row % a.q_heads), lane = threadIdx.x & 31;
+  if (a.c.length(s) == 0) {
+    *reinterpret_cast<uint2*>(a.out + row * 128 + lane * 4) = make_uint2(0u, 0u);
+    return;
   }
-  const float inv = 1.f / sum;
-  *reinterpret_cast<uint2*>(a.out + warp * 128 + lane * 4) =
-      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  const int group = a.q_heads / a.c.kv_heads, per_block = 2 * shared.per_tile;
+  const int block = s / per_block, in_block = s % per_block, tile = in_block / shared.per_tile;
+  Parts parts[2];
+  parts[0].base = shared.records;
+  parts[0].rows = 256;
+  parts[0].row = tile * 128 + (in_block - tile * shared.per_tile) * group + head % group;
+  parts[0].find((static_cast<int64_t>(block) * a.c.kv_heads + head / group) * shared.tiles, shared.tiles, shared.units,
+                shared.ctas);
+  if (parts[0].lo == parts[0].hi) parts[0].single(shared.whole + row * kRecord);
+  parts[1] = decode_parts(a, ctas, s, head);
+  join_parts(parts, a.out + row * 128);
 }
 
 size_t offsets_bytes(int sequences) { return ((static_cast<size_t>(sequences) + 1) * sizeof(int64_t) + 255) / 256 * 256; }
+
+DecodeArgs decode_args(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out, int q_heads,
+                       void* workspace) {
+  DecodeArgs a{};
+  a.c = c;
+  a.q = static_cast<const bf16*>(q);
+  a.k = static_cast<const bf16*>(k_pages);
+  a.v = static_cast<const bf16*>(v_pages);
+  a.out = static_cast<bf16*>(out);
+  a.offsets = static_cast<int64_t*>(workspace);
+  a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + offsets_bytes(c.sequences));
+  a.q_heads = q_heads;
+  return a;
+}
+
+int decode_grid(const PagedCache& c) {
+  const int64_t capacity = static_cast<int64_t>(c.max_pages - c.prefix_count) << c.page_shift;
+  const int64_t most = static_cast<int64_t>(c.sequences) * c.kv_heads * ((capacity + kUnit - 1) / kUnit);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kCtasPerSm * sm_count(), most)));
+}
+
+dim3 merge_grid(const PagedCache& c, int q_heads) {
+  return dim3(static_cast<unsigned>((static_cast<int64_t>(c.sequences) * q_heads + kWarps - 1) / kWarps));
+}
 
 }  // namespace
 
@@ -347,24 +377,41 @@ cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* 
   cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
-  DecodeArgs a{};
-  a.c = c;
-  a.q = static_cast<const bf16*>(q);
-  a.k = static_cast<const bf16*>(k_pages);
-  a.v = static_cast<const bf16*>(v_pages);
-  a.out = static_cast<bf16*>(out);
-  a.offsets = static_cast<int64_t*>(workspace);
-  a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + offsets_bytes(c.sequences));
-  a.q_heads = q_heads;
-  const int64_t capacity = static_cast<int64_t>(c.max_pages) << c.page_shift;
-  const int64_t most = static_cast<int64_t>(c.sequences) * c.kv_heads * ((capacity + kUnit - 1) / kUnit);
-  const int grid = static_cast<int>(std::min<int64_t>(kCtasPerSm * sm_count(), most));
+  const DecodeArgs a = decode_args(c, q, k_pages, v_pages, out, q_heads, workspace);
+  const int grid = decode_grid(c);
   paged_decode_kernel<<<grid, kThreads, kSmem, stream>>>(a);
   e = cudaGetLastError();
-  if (e != cudaSuccess || capacity <= kUnit) return e;  // one unit per item: nothing to merge
-  const int64_t warps = static_cast<int64_t>(c.sequences) * q_heads;
-  return launch_pdl(paged_decode_merge_kernel, dim3(static_cast<unsigned>((warps + kWarps - 1) / kWarps)), dim3(kThreads),
-                    0, stream, a, grid);
+  if (e != cudaSuccess || (c.max_pages << c.page_shift) <= kUnit) return e;  // one unit per item: nothing to merge
+  return launch_pdl(paged_decode_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a, grid);
+}
+
+size_t shared_prefix_workspace_bytes(const PagedCache& c, int q_heads) {
+  const size_t rows = static_cast<size_t>(c.sequences) * q_heads * kRecord * sizeof(float);
+  return 2 * rows + static_cast<size_t>(shared_keys_plan(c, q_heads).ctas) * 2 * 256 * kRecord * sizeof(float) +
+         paged_decode_workspace_bytes(c.sequences, q_heads, c.kv_heads);
+}
+
+cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
+                                 int q_heads, void* workspace, cudaStream_t stream) {
+  if (c.prefix_count == 0) return launch_paged_decode(c, q, k_pages, v_pages, out, q_heads, workspace, stream);
+  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(kSmem));
+  if (e != cudaSuccess) return e;
+  const size_t rows = static_cast<size_t>(c.sequences) * q_heads * kRecord;
+  SharedKeys shared = shared_keys_plan(c, q_heads);
+  DecodeArgs a = decode_args(c, q, k_pages, v_pages, out, q_heads, workspace);
+  shared.whole = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
+                                          paged_decode_workspace_bytes(c.sequences, q_heads, c.kv_heads));
+  a.whole = shared.whole + rows;
+  shared.records = a.whole + rows;
+  a.first = c.prefix_count << c.page_shift;
+  e = launch_shared_keys(c, q, k_pages, v_pages, q_heads, shared, stream);
+  if (e != cudaSuccess) return e;
+  // the sequences' own keys: nothing of it waits for the kernel before, so its CTAs start as that one's end
+  const int grid = decode_grid(c);
+  e = launch_pdl(paged_decode_kernel, dim3(grid), dim3(kThreads), kSmem, stream, a);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(shared_prefix_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a, grid, shared);
 }
 
 }  // namespace ipe

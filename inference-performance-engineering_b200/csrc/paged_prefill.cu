@@ -25,7 +25,7 @@
 #include <algorithm>
 
 #include "launch.h"
-#include "paged.cuh"
+#include "paged_records.cuh"
 #include "tensor_map.h"
 
 namespace ipe {
@@ -39,8 +39,6 @@ constexpr int kTile = 2 * kHalf;
 constexpr int kStages = 4;           // K or V tiles in flight
 constexpr int kTmemCols = 512;       // S0 [0, 128), S1 [128, 256), O0 [256, 384), O1 [384, 512)
 constexpr int kMaxListed = 1024;     // sequences (and, in runs, blocks) listed in shared memory
-constexpr int kRecord = 132;         // floats: o[128], maximum, sum, 2 unused
-constexpr float kScaleLog2 = 0.08838834764831845f * 1.4426950408889634f;  // 128^-0.5 * log2(e)
 constexpr float kSlack = 8.f / kScaleLog2;  // how far scores may pass the maximum in use
 
 struct Work {       // one piece: key tiles of a block
@@ -52,7 +50,7 @@ struct Work {       // one piece: key tiles of a block
   int keys;         // the block's keys: tiles end here
   int tile0;        // first key tile of the piece
   int count[2];     // key tiles of each query tile in this piece
-  int record;       // where the piece's rows go: -1 the output, else a record slot
+  int record;       // the record slot of a part, -1 for a whole block
 };
 
 struct Shared {
@@ -76,8 +74,10 @@ struct PrefillArgs {
   bf16* out;
   float* records;  // [grid][2][256][kRecord] where the key tiles are dealt in runs, else null
   int* lists;      // [2][kMaxListed + 1]: blocks before each sequence, key tiles before each block
+  float* whole;    // shared keys: where rows that are not in parts go, [tokens][q_heads][kRecord]
   int tokens;
   int q_heads;
+  int shared_keys;
 };
 
 // K-major operand, 128-byte swizzle: 8-row groups 1024 bytes apart.
@@ -151,12 +151,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // A row key by key, by a whole warp: o (4 dimensions per lane), maximum and sum over keys [from, to).
@@ -252,6 +246,10 @@ __device__ int block_scan(int x, int* warp_sums, int* total) {
   return before + scan - x;
 }
 
+// kShared: the "new tokens" are one query token of each sequence, all on the pages of c.prefix_pages (a
+// row sees those of them that its sequence's length covers), key tiles dealt in runs, and all rows go to
+// records that the decode kernel's merge joins with the rest of each sequence.
+template <bool kShared>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PrefillArgs a) {
@@ -266,7 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.q_heads / c.kv_heads;
   const int per_tile = kBM / group, per_block = 2 * per_tile;  // tokens
-  const bool in_runs = a.records != nullptr;
+  const bool in_runs = kShared || a.records != nullptr;
+  pdl_trigger();
 
   if (threadIdx.x == 0) {
     mbar_init(&sh.q_full, 1);
@@ -294,8 +293,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // In runs: sh.low = blocks before each sequence, sh.high = key tiles before each block. Otherwise
   // sh.low .. sh.high: the sequence's blocks as numbers that grow with their keys (block 0 of a sequence
   // on a context starts at the context's length in blocks).
-  int blocks = 0;
-  for (int base = 0; base < c.sequences; base += kThreads) {
+  const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
+  int blocks = kShared ? (a.tokens + per_block - 1) / per_block : 0;
+  for (int base = 0; !kShared && base < c.sequences; base += kThreads) {
     const int s = base + threadIdx.x;
     Span x{0, 0, 0};
     if (s < c.sequences) x = span_of(c, s, a.tokens);
@@ -309,8 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     blocks += all;
   }
-  int tiles = 0;
-  if (in_runs) {
+  int tiles = kShared ? blocks * shared_tiles : 0;
+  if (!kShared && in_runs) {
     blocks = min(blocks, kMaxListed);
     const int listed = min(c.sequences, kMaxListed);
     if (threadIdx.x == 0) sh.low[listed] = blocks;
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   const int64_t units = static_cast<int64_t>(tiles) * c.kv_heads;
-  const int runs = static_cast<int>(min(units, static_cast<int64_t>(gridDim.x)));
+  const int runs = runs_of(units, gridDim.x);
 
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ work list and loads
@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t works = static_cast<int64_t>(blocks) * c.kv_heads;
     int64_t unit = 0, unit_end = 0;  // in runs
     if (in_runs && static_cast<int>(blockIdx.x) < runs) {
-      unit = units * blockIdx.x / runs;
-      unit_end = units * (blockIdx.x + 1) / runs;
+      unit = run_start(units, blockIdx.x, runs);
+      unit_end = run_start(units, blockIdx.x + 1, runs);
     }
     const bool listed = c.sequences <= kMaxListed;
     auto range_of = [&](int s, int* low, int* high) {
@@ -418,22 +418,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (in_runs) {
         if (unit >= unit_end) break;
         int lo = 0, hi = blocks;  // the block of this unit: the last with high[i] * kv_heads <= unit
+        if (kShared) {
+          lo = static_cast<int>(unit / (static_cast<int64_t>(shared_tiles) * c.kv_heads));
+          hi = lo + 1;
+        }
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
           if (static_cast<int64_t>(sh.high[mid]) * c.kv_heads <= unit) lo = mid;
           else hi = mid;
         }
-        const int block = lo, n = sh.high[block + 1] - sh.high[block];
-        const int r = static_cast<int>(unit - static_cast<int64_t>(sh.high[block]) * c.kv_heads);
+        const int block = lo, before = kShared ? block * shared_tiles : sh.high[block];
+        const int n = kShared ? shared_tiles : sh.high[block + 1] - before;
+        const int r = static_cast<int>(unit - static_cast<int64_t>(before) * c.kv_heads);
         const int tile0 = r % n, tile1 = static_cast<int>(min(static_cast<int64_t>(n), tile0 + unit_end - unit));
-        lo = 0;
-        hi = min(c.sequences, kMaxListed);
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (sh.low[mid] <= block) lo = mid;
-          else hi = mid;
+        if (kShared) {
+          // every row sees up to all shared keys: as if the tokens stood behind them
+          w = make_work(Span{0, a.tokens, a.shared_keys + a.tokens}, 0, block, r / n, per_tile, tile0, tile1);
+          w.keys = a.shared_keys;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) w.count[i] = w.tokens > i * per_tile ? tile1 - tile0 : 0;
+        } else {
+          lo = 0;
+          hi = min(c.sequences, kMaxListed);
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (sh.low[mid] <= block) lo = mid;
+            else hi = mid;
+          }
+          w = make_work(span_of(c, lo, a.tokens), lo, block - sh.low[lo], r / n, per_tile, tile0, tile1);
         }
-        w = make_work(span_of(c, lo, a.tokens), lo, block - sh.low[lo], r / n, per_tile, tile0, tile1);
         if (tile0 > 0 || tile1 < n) w.record = static_cast<int>(blockIdx.x) * 2 + (round == 0 ? 0 : 1);
         unit += tile1 - tile0;
       } else {
@@ -636,7 +649,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int count = w.count[i];
       const int token = i * per_tile + place;
       const bool real = place < per_tile && token < w.tokens;
-      const int limit = real ? max(0, w.position0 + token + 1) : 0;  // keys the row sees
+      int limit = 0;  // keys the row sees
+      if (real) limit = kShared ? min(c.length(w.token0 + token), a.shared_keys) : max(0, w.position0 + token + 1);
       float m = -INFINITY, l = 0.f;
       for (int step = 0; step < count && ok; ++step) {
         if (!wait_all(&sh.s_full[i], s_seen & 1)) {
@@ -705,7 +719,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const int64_t out_row = static_cast<int64_t>(w.token0 + token) * a.q_heads + w.kv_head * group + head;
-      float* rec = w.record < 0 ? nullptr : a.records + (static_cast<int64_t>(w.record) * 2 * kBM + i * kBM + r) * kRecord;
+      float* rec = w.record >= 0 ? a.records + (static_cast<int64_t>(w.record) * 2 * kBM + i * kBM + r) * kRecord
+                   : kShared    ? a.whole + out_row * kRecord
+                                : nullptr;
       const float inv = limit > 0 ? 1.f / l : 0.f;
       bool finite = true;
       if (count > 0) {
@@ -751,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float o[4], top, sum;
         attend_row(c, a.q + row * 128, a.k, a.v, w.sequence, w.kv_head, first, min(keys, first + count * kBN), o, &top, &sum);
         if (rec) {
-          float* at = rec + (from - lane) * kRecord;
+          float* at = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(rec), from));
           *reinterpret_cast<float4*>(at + lane * 4) = make_float4(o[0], o[1], o[2], o[3]);
           if (lane == 0) {
             at[128] = top;
@@ -795,38 +811,18 @@ __global__ void __launch_bounds__(128) paged_prefill_merge_kernel(const PrefillA
   const int* before = a.lists + kMaxListed + 1;
   const int tile0 = __ldcg(before + block), n = __ldcg(before + block + 1) - tile0;
   const int64_t units = static_cast<int64_t>(__ldcg(before + blocks)) * c.kv_heads;
-  const int runs = static_cast<int>(min(units, static_cast<int64_t>(ctas)));
-  const int64_t first = static_cast<int64_t>(tile0) * c.kv_heads + static_cast<int64_t>(head / group) * n;
-  const int run_lo = static_cast<int>(((first + 1) * runs - 1) / units);
-  const int run_hi = static_cast<int>(((first + n) * runs - 1) / units);
-  if (run_lo == run_hi) return;  // whole, already written
-  const int slot_lo = units * run_lo / runs == first ? 0 : 1;
+  Parts parts[1];
+  parts[0].base = a.records;
+  parts[0].rows = 2 * kBM;
   const int in_block = place % per_block, tile = in_block / per_tile;
-  const int r = tile * kBM + (in_block - tile * per_tile) * group + head % group;
-  auto record = [&](int run) {
-    return a.records + ((static_cast<int64_t>(run) * 2 + (run == run_lo ? slot_lo : 0)) * 2 * kBM + r) * kRecord;
-  };
-  float top = -INFINITY;
-  for (int run = run_lo + lane; run <= run_hi; run += 32) top = fmaxf(top, __ldcg(record(run) + 128));
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
-  float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int run = run_lo; run <= run_hi; ++run) {
-    const float* rec = record(run);
-    const float4 y = __ldcg(reinterpret_cast<const float4*>(rec) + lane);
-    const float e = exp2_approx(__ldcg(rec + 128) * kScaleLog2 - base);
-    sum += e * __ldcg(rec + 129);
-    o.x += e * y.x;
-    o.y += e * y.y;
-    o.z += e * y.z;
-    o.w += e * y.w;
-  }
-  const float inv = x.length - x.tokens + place >= 0 ? 1.f / sum : 0.f;  // no position: no keys
-  const bool none = inv == 0.f && x.length - x.tokens + place < 0;
-  *reinterpret_cast<uint2*>(a.out + warp * 128 + lane * 4) =
-      none ? make_uint2(0u, 0u) : make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  parts[0].row = tile * kBM + (in_block - tile * per_tile) * group + head % group;
+  parts[0].find(static_cast<int64_t>(tile0) * c.kv_heads + static_cast<int64_t>(head / group) * n, n, units, ctas);
+  if (parts[0].lo == parts[0].hi) return;  // whole, already written
+  bf16* row = a.out + warp * 128;
+  if (x.length - x.tokens + place < 0)  // no position: no keys
+    *reinterpret_cast<uint2*>(row + lane * 4) = make_uint2(0u, 0u);
+  else
+    join_parts(parts, row);
 }
 
 constexpr size_t kListBytes = (2 * (kMaxListed + 1) * sizeof(int) + 255) / 256 * 256;
@@ -850,39 +846,83 @@ size_t paged_prefill_workspace_bytes(int64_t tokens, int sequences, int q_heads,
   return kListBytes + static_cast<size_t>(sm_count()) * 2 * 2 * kBM * kRecord * sizeof(float);
 }
 
-cudaError_t launch_paged_prefill(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
-                                 int64_t tokens, int q_heads, void* workspace, cudaStream_t stream) {
+namespace {
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+// The tensor maps and arguments that both launches share.
+cudaError_t prepare(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, int64_t tokens,
+                    int q_heads, Maps* maps, PrefillArgs* a) {
   const int group = q_heads / c.kv_heads, page_size = 1 << c.page_shift;
   const int rows = static_cast<int>(static_cast<int64_t>(c.num_pages) * c.kv_heads * page_size);
-  CUtensorMap mq, mk, mv;
-  if (!make_map_3d(&mq, q, kD, q_heads, static_cast<int>(tokens), q_heads, group, 64, kBM / group) ||
-      !make_map_2d(&mk, k_pages, rows, kD, page_size, 64) || !make_map_2d(&mv, v_pages, rows, kD, page_size, 64))
+  if (!make_map_3d(&maps->q, q, kD, q_heads, static_cast<int>(tokens), q_heads, group, 64, kBM / group) ||
+      !make_map_2d(&maps->k, k_pages, rows, kD, page_size, 64) || !make_map_2d(&maps->v, v_pages, rows, kD, page_size, 64))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  *a = PrefillArgs{};
+  a->c = c;
+  a->q = static_cast<const bf16*>(q);
+  a->k = static_cast<const bf16*>(k_pages);
+  a->v = static_cast<const bf16*>(v_pages);
+  a->tokens = static_cast<int>(tokens);
+  a->q_heads = q_heads;
+  return cudaSuccess;
+}
+
+template <bool kShared>
+cudaError_t launch(int64_t grid, const Maps& maps, const PrefillArgs& a, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(kSmem));
   if (e != cudaSuccess) return e;
-  PrefillArgs a{};
-  a.c = c;
-  a.q = static_cast<const bf16*>(q);
-  a.k = static_cast<const bf16*>(k_pages);
-  a.v = static_cast<const bf16*>(v_pages);
+  paged_prefill_kernel<kShared><<<static_cast<unsigned>(grid), kThreads, kSmem, stream>>>(maps.q, maps.k, maps.v, a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_paged_prefill(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
+                                 int64_t tokens, int q_heads, void* workspace, cudaStream_t stream) {
+  Maps maps;
+  PrefillArgs a;
+  cudaError_t e = prepare(c, q, k_pages, v_pages, tokens, q_heads, &maps, &a);
+  if (e != cudaSuccess) return e;
   a.out = static_cast<bf16*>(out);
-  a.tokens = static_cast<int>(tokens);
-  a.q_heads = q_heads;
   const bool in_runs = deal_in_runs(tokens, c.sequences, q_heads, c.kv_heads);
-  int64_t grid = most_blocks(tokens, c.sequences, group) * c.kv_heads;
+  int64_t grid = most_blocks(tokens, c.sequences, q_heads / c.kv_heads) * c.kv_heads;
   if (in_runs) {
     a.lists = static_cast<int*>(workspace);
     a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kListBytes);
-    grid *= std::max<int64_t>(1, ((static_cast<int64_t>(c.max_pages) << c.page_shift) + kBN - 1) / kBN);
+    grid *= ((static_cast<int64_t>(c.max_pages) << c.page_shift) + kBN - 1) / kBN;
   }
   grid = std::min<int64_t>(grid, sm_count());
-  paged_prefill_kernel<<<static_cast<unsigned>(grid), kThreads, kSmem, stream>>>(mq, mk, mv, a);
-  e = cudaGetLastError();
+  e = launch<false>(grid, maps, a, stream);
   if (e != cudaSuccess || !in_runs) return e;
   const int64_t warps = tokens * q_heads;
   return launch_pdl(paged_prefill_merge_kernel, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, stream, a,
                     static_cast<int>(grid));
+}
+
+SharedKeys shared_keys_plan(const PagedCache& c, int q_heads) {
+  SharedKeys p{};
+  p.per_tile = kBM / (q_heads / c.kv_heads);
+  p.tiles = ((c.prefix_count << c.page_shift) + kBN - 1) / kBN;
+  const int64_t blocks = (c.sequences + 2 * p.per_tile - 1) / (2 * p.per_tile);
+  p.units = blocks * c.kv_heads * p.tiles;
+  p.ctas = static_cast<int>(std::min<int64_t>(p.units, sm_count()));
+  return p;
+}
+
+cudaError_t launch_shared_keys(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, int q_heads,
+                               const SharedKeys& plan, cudaStream_t stream) {
+  Maps maps;
+  PrefillArgs a;
+  cudaError_t e = prepare(c, q, k_pages, v_pages, c.sequences, q_heads, &maps, &a);
+  if (e != cudaSuccess) return e;
+  a.records = plan.records;
+  a.whole = plan.whole;
+  a.shared_keys = c.prefix_count << c.page_shift;
+  return launch<true>(plan.ctas, maps, a, stream);
 }
 
 }  // namespace ipe

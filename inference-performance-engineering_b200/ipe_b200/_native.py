@@ -55,7 +55,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                             c_int, _P, c_size_t, _P]),
     "ipe_paged_prefill_attention_workspace": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "ipe_shared_prefix_attention": (c_int, [_P, _P, _P, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int64, c_int,
-                                            c_int, _P]),
+                                            c_int, _P, c_size_t, _P]),
+    "ipe_shared_prefix_attention_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "ipe_gemm": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, _P]),
     "ipe_decode_step": (c_int, [ctypes.c_void_p, _P]),
     "ipe_decode_step_workspace": (c_size_t, [c_int, c_int, c_int, c_int]),

@@ -170,7 +170,10 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     if prefix_pages.dim() != 1 or prefix_pages.shape[0] > width:
         raise ValueError(f"{name}: prefix_pages must be [prefix pages], no more than the {width} pages per sequence")
     with _on(device):
+        ws = _workspace(device, "ipe_shared_prefix_attention_workspace", sequences, q_heads, kv_heads, page_size,
+                        prefix_pages.shape[0])
         nat.call("ipe_shared_prefix_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                  prefix_pages.data_ptr(), prefix_pages.shape[0], page_table.data_ptr(), lengths.data_ptr(),
-                 out.data_ptr(), sequences, q_heads, kv_heads, pages, page_size, width, _stream(device))
+                 out.data_ptr(), sequences, q_heads, kv_heads, pages, page_size, width, ws.data_ptr(), ws.numel(),
+                 _stream(device))
     return out
