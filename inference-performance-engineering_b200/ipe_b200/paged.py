@@ -35,12 +35,18 @@ from ipe_b200 import _native as nat
 _SAME_DEVICE = contextlib.nullcontext()
 
 
-def _check(name: str, device: torch.device, **tensors: tuple[torch.Tensor, torch.dtype]) -> None:
-    """Every tensor is contiguous, on `device` and of the dtype beside it."""
-    for label, (t, dtype) in tensors.items():
-        if not isinstance(t, torch.Tensor) or t.device != device or device.type != "cuda":
+def _device(name: str, pages: torch.Tensor) -> int:
+    if not isinstance(pages, torch.Tensor) or not pages.is_cuda:
+        raise ValueError(f"{name}: expected CUDA tensors")
+    return pages.get_device()
+
+
+def _check(name: str, device: int, dtype: torch.dtype, **tensors: torch.Tensor) -> None:
+    """Every tensor is contiguous, on CUDA device `device` and of `dtype`."""
+    for label, t in tensors.items():
+        if not isinstance(t, torch.Tensor) or t.get_device() != device:
             raise ValueError(f"{name}: {label} must be a CUDA tensor, on the device of the others")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise ValueError(f"{name}: {label} must be {dtype}, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{name}: {label} must be contiguous")
@@ -65,23 +71,23 @@ def _heads(name: str, q: torch.Tensor, out: torch.Tensor, rows: int | None = Non
     return q.shape[1]
 
 
-def _on(device: torch.device):
+def _on(device: int):
     """The guard under which a call's stream, workspace and launches belong to `device`."""
-    return _SAME_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _SAME_DEVICE if device == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def _stream(device: torch.device) -> int:
+def _stream(device: int) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(entry: str, device_index: int, *sizes: int) -> int:
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(entry: str, device: int, *sizes: int) -> int:
     return int(getattr(nat.load(), entry)(*sizes))
 
 
-def _workspace(device: torch.device, entry: str, *sizes: int) -> torch.Tensor:
+def _workspace(device: int, entry: str, *sizes: int) -> torch.Tensor:
     """The call's own scratch, from torch's allocator: calls on other streams, and captured ones, have others."""
-    return torch.empty(_workspace_bytes(entry, device.index, *sizes), dtype=torch.uint8, device=device)
+    return torch.empty(_workspace_bytes(entry, device, *sizes), dtype=torch.uint8, device=device)
 
 
 def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor,
@@ -95,11 +101,11 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: t
     sets device error 2, and its row is skipped.
     """
     name = "paged_qk_norm_rope_append"
-    bf16, device = torch.bfloat16, getattr(k_pages, "device", torch.device("cpu"))
-    table = cos.dtype if getattr(cos, "dtype", None) == torch.float32 else bf16
-    _check(name, device, qkv=(qkv, bf16), q_norm=(q_norm, bf16), k_norm=(k_norm, bf16), cos=(cos, table),
-           sin=(sin, table), cu_tokens=(cu_tokens, torch.int32), lengths=(lengths, torch.int32),
-           page_table=(page_table, torch.int32), q_out=(q_out, bf16), k_pages=(k_pages, bf16), v_pages=(v_pages, bf16))
+    device = _device(name, k_pages)
+    table = torch.float32 if getattr(cos, "dtype", None) is torch.float32 else torch.bfloat16
+    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, qkv=qkv, q_norm=q_norm, k_norm=k_norm, q_out=q_out)
+    _check(name, device, table, cos=cos, sin=sin)
+    _check(name, device, torch.int32, cu_tokens=cu_tokens, lengths=lengths, page_table=page_table)
     pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
     if q_out.dim() != 3 or q_out.shape[2] != 128 or qkv.shape != (q_out.shape[0], (q_out.shape[1] + 2 * kv_heads) * 128):
         raise ValueError(f"{name}: qkv must be [rows, (query heads + 2 * KV heads) * 128] and q_out [rows, query heads, 128]")
@@ -109,7 +115,7 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: t
         raise ValueError(f"{name}: cu_tokens must be [sequences + 1]")
     with _on(device):
         nat.call("ipe_paged_qk_norm_rope_append", qkv.data_ptr(), q_out.shape[0], q_out.shape[1], kv_heads,
-                 q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), int(table == torch.float32),
+                 q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), int(table is torch.float32),
                  cos.shape[0], cu_tokens.data_ptr(), lengths.data_ptr(), page_table.data_ptr(), sequences, width,
                  q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size, float(eps), _stream(device))
     return q_out
@@ -120,9 +126,9 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """out [S, Hq * 128] = softmax(q k^T / sqrt(128)) v over keys 0 .. lengths[s] - 1 of every sequence, one query
     token q [S, Hq, 128] each, 1 to 8 query heads per KV head. A sequence of length 0 gives zeros."""
     name = "paged_decode_attention"
-    bf16, device = torch.bfloat16, getattr(k_pages, "device", torch.device("cpu"))
-    _check(name, device, q=(q, bf16), k_pages=(k_pages, bf16), v_pages=(v_pages, bf16),
-           page_table=(page_table, torch.int32), lengths=(lengths, torch.int32), out=(out, bf16))
+    device = _device(name, k_pages)
+    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
+    _check(name, device, torch.int32, page_table=page_table, lengths=lengths)
     pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
     q_heads = _heads(name, q, out, sequences)
     with _on(device):
@@ -138,10 +144,9 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     """Causal attention of ragged new tokens q [rows, Hq, 128] over their sequences' pages: token i of the n that
     sequence s brings sees keys 0 .. lengths[s] - n + i. out [rows, Hq * 128]; 1 to 8 query heads per KV head."""
     name = "paged_prefill_attention"
-    bf16, device = torch.bfloat16, getattr(k_pages, "device", torch.device("cpu"))
-    _check(name, device, q=(q, bf16), k_pages=(k_pages, bf16), v_pages=(v_pages, bf16),
-           page_table=(page_table, torch.int32), cu_tokens=(cu_tokens, torch.int32), lengths=(lengths, torch.int32),
-           out=(out, bf16))
+    device = _device(name, k_pages)
+    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
+    _check(name, device, torch.int32, page_table=page_table, cu_tokens=cu_tokens, lengths=lengths)
     pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
     q_heads = _heads(name, q, out)
     if cu_tokens.shape != (sequences + 1,):
@@ -161,10 +166,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     sequence] is read for the positions behind it alone (its first prefix_pages.numel() columns may hold anything).
     lengths [S] count the prefix; a sequence that ends inside the prefix sees its own lengths[s] keys of it."""
     name = "shared_prefix_attention"
-    bf16, device = torch.bfloat16, getattr(k_pages, "device", torch.device("cpu"))
-    _check(name, device, q=(q, bf16), k_pages=(k_pages, bf16), v_pages=(v_pages, bf16),
-           prefix_pages=(prefix_pages, torch.int32), page_table=(page_table, torch.int32), lengths=(lengths, torch.int32),
-           out=(out, bf16))
+    device = _device(name, k_pages)
+    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
+    _check(name, device, torch.int32, prefix_pages=prefix_pages, page_table=page_table, lengths=lengths)
     pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
     q_heads = _heads(name, q, out, sequences)
     if prefix_pages.dim() != 1 or prefix_pages.shape[0] > width:
