@@ -36,15 +36,18 @@ struct PagedCache {
     report(err, kErrPositionRange);
     return 0;
   }
-  // the page of a position below length(s); a page outside the cache sets device error 5 and reads
-  // as page 0, so nothing outside the cache is touched
-  __device__ __forceinline__ int page(int s, int position) const {
+  // what the tables say of a position below length(s), not looked at
+  __device__ __forceinline__ int page_id(int s, int position) const {
     const int j = position >> page_shift;
-    const int id = j < prefix_count ? __ldg(prefix_pages + j) : __ldg(page_table + static_cast<int64_t>(s) * max_pages + j);
+    return j < prefix_count ? __ldg(prefix_pages + j) : __ldg(page_table + static_cast<int64_t>(s) * max_pages + j);
+  }
+  // a page outside the cache sets device error 5 and reads as page 0, so nothing outside the cache is touched
+  __device__ __forceinline__ int checked(int id) const {
     if (static_cast<unsigned>(id) < static_cast<unsigned>(num_pages)) return id;
     report(err, kErrPage);
     return 0;
   }
+  __device__ __forceinline__ int page(int s, int position) const { return checked(page_id(s, position)); }
   // first row (of 128 elements) of a page's head
   __device__ __forceinline__ int64_t page_row(int page_id, int kv_head) const {
     return (static_cast<int64_t>(page_id) * kv_heads + kv_head) << page_shift;

@@ -31,14 +31,17 @@
 namespace ipe {
 namespace {
 
-constexpr int kThreads = 320;
-constexpr int kLoadWarp = 8, kMmaWarp = 9;  // warps 0-7: softmax
+constexpr int kThreads = 384;      // three warpgroups: softmax of query tile 0, of tile 1, and the rest
+constexpr int kLoadWarp = 8, kMmaWarp = 9;  // warps 0-7: softmax; 10, 11 idle
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 2 * 208 + 88 = 3 * 168, what the launch holds
 constexpr int kBM = 128, kBN = 128, kD = 128;
 constexpr int kHalf = 128 * 64 * 2;  // a 128-row x 64-column bf16 block, 128-byte swizzle
 constexpr int kTile = 2 * kHalf;
-constexpr int kStages = 4;           // K or V tiles in flight
-constexpr int kTmemCols = 512;       // S0 [0, 128), S1 [128, 256), O0 [256, 384), O1 [384, 512)
+constexpr int kStages = 2;           // pairs of tiles in the ring: the values of a step and the keys of the next
+constexpr int kTmemCols = 512;       // all there are, so they begin at column
+constexpr uint32_t kTmem = 0;        // S0 [0, 128), S1 [128, 256), O0 [256, 384), O1 [384, 512)
 constexpr int kMaxListed = 1024;     // sequences (and, in runs, blocks) listed in shared memory
+constexpr int kByCubic = 1;          // of every 4 pairs of weights, those whose 2^x is a cubic
 constexpr float kSlack = 8.f / kScaleLog2;  // how far scores may pass the maximum in use
 
 struct Work {       // one piece: key tiles of a block
@@ -55,8 +58,8 @@ struct Work {       // one piece: key tiles of a block
 
 struct Shared {
   uint64_t q_full, q_empty;
-  uint64_t kv_full[kStages], kv_empty[kStages];
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t pair_full[kStages], pair_empty[kStages];
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
   uint32_t tmem;
   int abort;
   int blocks;
@@ -64,7 +67,7 @@ struct Shared {
   Work work[2];
   int low[kMaxListed + 1], high[kMaxListed + 1];
 };
-constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + kStages) * kTile + sizeof(Shared);
+constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + 2 * kStages) * kTile + sizeof(Shared);
 
 struct PrefillArgs {
   PagedCache c;
@@ -80,32 +83,34 @@ struct PrefillArgs {
   int shared_keys;
 };
 
-// K-major operand, 128-byte swizzle: 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
-// MN-major operand (V: the head's dimensions contiguous): 64-column halves kHalf apart, 8-key groups 1024.
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kHalf >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Shared-memory operands with the 128-byte swizzle, 8-row groups 1024 bytes apart. The upper words of
+// their descriptors are alike; the lower ones hold the address, and for an MN-major operand (V: the
+// head's dimensions contiguous) the distance of its 64-column halves.
+constexpr uint32_t kDescUpper = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mnmajor(uint32_t addr) { return (addr >> 4) | (static_cast<uint32_t>(kHalf >> 4) << 16); }
 // kind::f16: fp32 D, bf16 A and B, M = N = 128; B transposed (MN-major) when transpose_b.
 __device__ __forceinline__ constexpr uint32_t instr_desc(bool transpose_b) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (transpose_b ? (1u << 16) : 0u) | (static_cast<uint32_t>(kBN >> 3) << 17) |
          (static_cast<uint32_t>(kBM >> 4) << 24);
 }
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescUpper));
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescUpper));
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
@@ -153,8 +158,76 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+// Bounded waits of a whole converged warp, the same answer in every lane. The first try is all that is
+// inline: a warp that finds the phase complete, as the MMA warp mostly does, goes through few instructions.
+__device__ __forceinline__ bool wait_longer(uint64_t* bar, uint32_t parity, int* err) {
+  uint64_t start = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((i & 63u) == 0) {
+      const uint64_t now = __shfl_sync(0xffffffffu, globaltimer_ns(), 0);
+      if (start == 0) start = now;
+      if (now - start > kWaitLimitNs) {
+        report(err, kErrWaitTimeout);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_longer(bar, parity, err);
+}
+
+// Pairs of fp32 in one 64-bit register: two operations per instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float* lo, float* hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the largest of three; NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x for a pair, without the special function unit, which is the busiest: x = n + f, n the nearest
+// integer, 2^f on [-1/2, 1/2] by the cubic through 1 of least largest relative error (1.02e-4, fitted by
+// iteratively reweighted least squares; a bf16 weight is off by up to 3.9e-3), n added to the exponent.
+// x below -127 counts as -127, where the exponent field and the cubic's fraction reach zero together: a
+// hidden key's weight is exactly 0, as it has to be beside a value of the type's largest.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float* p0, float* p1) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest integer in the low bits
+  float lo, hi;
+  unpair(x, &lo, &hi);
+  x = pair(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
+  const uint64_t n = add2(x, pair(kRound, kRound));
+  const uint64_t f = fma2(add2(n, pair(-kRound, -kRound)), pair(-1.f, -1.f), x);
+  uint64_t y = fma2(pair(0.0550089329f, 0.0550089329f), f, pair(0.242210969f, 0.242210969f));
+  y = fma2(y, f, pair(0.693282902f, 0.693282902f));
+  y = fma2(y, f, pair(1.f, 1.f));
+  float n0, n1, y0, y1;
+  unpair(n, &n0, &n1);
+  unpair(y, &y0, &y1);
+  *p0 = __int_as_float((__float_as_int(n0) << 23) + __float_as_int(y0));
+  *p1 = __int_as_float((__float_as_int(n1) << 23) + __float_as_int(y1));
+}
+
 // A row key by key, by a whole warp: o (4 dimensions per lane), maximum and sum over keys [from, to).
-__device__ __noinline__ void attend_row(const PagedCache& c, const bf16* q_row, const bf16* k, const bf16* v, int s,
+__device__ __forceinline__ void attend_row(const PagedCache& c, const bf16* q_row, const bf16* k, const bf16* v, int s,
                                         int kv_head, int from, int to, float* o, float* top, float* sum) {
   const int lane = threadIdx.x & 31;
   const uint2 raw = *reinterpret_cast<const uint2*>(q_row + lane * 4);
@@ -257,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* s_q = smem;
   unsigned char* ring = smem + 2 * kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(ring + kStages * kTile);
+  Shared& sh = *reinterpret_cast<Shared*>(ring + kStages * 2 * kTile);
   volatile int* abort_flag = &sh.abort;
   const PagedCache& c = a.c;
   int* err = c.err;
@@ -271,12 +344,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1 + 8);  // the last S of the piece, and every softmax warp's look at the list
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sh.kv_full[s], 1);
-      mbar_init(&sh.kv_empty[s], 1);
+      mbar_init(&sh.pair_full[s], 1);
+      mbar_init(&sh.pair_empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 128);
+      mbar_init(&sh.p_full[i][0], 128);  // the first and the second 64 keys
+      mbar_init(&sh.p_full[i][1], 128);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_empty[i], 128);
     }
@@ -344,10 +418,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  if (threadIdx.x == 0 && sh.tmem != kTmem) report(err, kErrShape);
   const int64_t units = static_cast<int64_t>(tiles) * c.kv_heads;
   const int runs = runs_of(units, gridDim.x);
 
+  if (warp >= kLoadWarp) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ work list and loads
     const int ps = c.page_size(), subs = kBN >> c.page_shift;
@@ -411,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     int slot = 0, piece = 0;
-    uint32_t phase = 0, armed = 0;  // bit s: parity armed on kv_full[s]; bit 16 + s: armed at all
+    uint32_t phase = 0, armed = 0;  // bit s: parity armed on pair_full[s]; bit 16 + s: armed at all
     bool ok = true;
     for (int64_t round = 0; ok && !*abort_flag; ++round, ++piece) {
       Work w;
@@ -460,8 +536,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         select(static_cast<int>(rank / c.kv_heads), &s, &b);
         w = make_work(span_of(c, s, a.tokens), s, b, static_cast<int>(rank % c.kv_heads), per_tile, 0, -1);
       }
-      if (!mbar_wait(&sh.q_empty, (piece & 1) ^ 1, err)) ok = false;
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
+        ok = false;
+        break;
+      }
       if (lane == 0) {
         sh.work[piece & 1] = w;
         const int rows = group * per_tile * 128;  // bytes of a query tile's half
@@ -474,42 +552,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const int steps = max(w.count[0], w.count[1]);
-      auto page_row = [&](int step) {  // this lane's part of the tile, -1 for none
-        const int key = (w.tile0 + step) * kBN + lane * ps;
-        if (lane >= subs || step >= steps || key >= w.keys) return -1;
-        return static_cast<int>(c.page_row(c.page(w.sequence, key), w.kv_head));
-      };
-      int row = page_row(0);
-      for (int step = 0; ok && step < steps; ++step) {
-        const int next = page_row(step + 1);
-        const int parts = __popc(__ballot_sync(0xffffffffu, row >= 0));
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!mbar_wait(&sh.kv_empty[slot], phase ^ 1, err)) ok = false;
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_expect_tx(&sh.kv_full[slot], parts * ps * 256);
-          __syncwarp();
-          if (row >= 0) {
-            const CUtensorMap* map = kv ? &map_v : &map_k;
-            const uint32_t dst = smem_addr(ring) + slot * kTile + lane * ps * 128;
-            tma_load_2d(dst, map, &sh.kv_full[slot], 0, row);
-            tma_load_2d(dst + kHalf, map, &sh.kv_full[slot], 64, row);
-          }
-          armed = (armed & ~(1u << slot)) | (phase << slot) | (1u << (16 + slot));
-          if (++slot == kStages) {
-            slot = 0;
-            phase ^= 1;
-          }
+      // This lane's page of a step's tile: its ID is loaded a step ahead and looked at when it is used.
+      auto key_of = [&](int step) { return (w.tile0 + step) * kBN + lane * ps; };
+      auto has_page = [&](int step) { return lane < subs && step < steps && key_of(step) < w.keys; };
+      auto load_id = [&](int step) { return has_page(step) ? c.page_id(w.sequence, key_of(step)) : 0; };
+      int id = load_id(0), row = 0, row_v = 0;  // cache rows of the keys to load, and of the step before
+      bool has = has_page(0), has_v = false;
+      for (int step = 0; step <= steps; ++step) {  // keys of `step`, values of the step before
+        if (has) row = static_cast<int>(c.page_row(c.checked(id), w.kv_head));
+        id = load_id(step + 1);
+        const int parts = __popc(__ballot_sync(0xffffffffu, has)) + __popc(__ballot_sync(0xffffffffu, has_v));
+        if (!wait_warp(&sh.pair_empty[slot], phase ^ 1, err)) {
+          ok = false;
+          break;
         }
-        row = next;
+        if (lane == 0) mbar_expect_tx(&sh.pair_full[slot], parts * ps * 256);
+        __syncwarp();
+        const uint32_t dst = smem_addr(ring) + slot * 2 * kTile + lane * ps * 128;
+        if (has_v) {
+          tma_load_2d(dst, &map_v, &sh.pair_full[slot], 0, row_v);
+          tma_load_2d(dst + kHalf, &map_v, &sh.pair_full[slot], 64, row_v);
+        }
+        if (has) {
+          tma_load_2d(dst + kTile, &map_k, &sh.pair_full[slot], 0, row);
+          tma_load_2d(dst + kTile + kHalf, &map_k, &sh.pair_full[slot], 64, row);
+        }
+        armed = (armed & ~(1u << slot)) | (phase << slot) | (1u << (16 + slot));
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1;
+        }
+        row_v = row;
+        has_v = has;
+        has = has_page(step + 1);
       }
     }
     if (!ok) *abort_flag = 1;
     // tell the others that the list has ended
-    if (ok && !*abort_flag && mbar_wait(&sh.q_empty, (piece & 1) ^ 1, err)) {
-      __syncwarp();
+    if (ok && !*abort_flag && wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
       if (lane == 0) {
         sh.work[piece & 1].token0 = -1;
         mbar_arrive(&sh.q_full);
@@ -520,65 +600,77 @@ __global__ void __launch_bounds__(kThreads, 1)
     // copies and arrivals in flight land before the CTA's shared memory goes away
     for (int s = 0; s < kStages; ++s) {
       if (!(armed & (1u << (16 + s)))) continue;
-      mbar_wait(&sh.kv_full[s], (armed >> s) & 1u, err);
-      if (!*abort_flag) mbar_wait(&sh.kv_empty[s], (armed >> s) & 1u, err);
+      mbar_wait(&sh.pair_full[s], (armed >> s) & 1u, err);
+      if (!*abort_flag) mbar_wait(&sh.pair_empty[s], (armed >> s) & 1u, err);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ MMA issue
-    const uint32_t idesc_s = instr_desc(false), idesc_o = instr_desc(true);
-    int it = 0;  // K and V tiles taken so far
+    // Everything an MMA is given is the same in all lanes and looks so to the compiler (constants, loop
+    // counters, warp reductions): operands that may differ cost it about 100 cycles per MMA.
+    constexpr uint32_t idesc_s = instr_desc(false), idesc_o = instr_desc(true);
+    const uint32_t q_desc = desc_kmajor(smem_addr(s_q)), k_desc = desc_kmajor(smem_addr(ring) + kTile),
+                   v_desc = desc_mnmajor(smem_addr(ring));
+    uint32_t it = 0;  // pairs taken so far
     uint32_t p_seen[2] = {0, 0}, o_seen[2] = {0, 0};
-    bool ok = true;
-    for (int piece = 0; ok && !*abort_flag; ++piece) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&sh.q_full, piece & 1, err))) {
-        ok = false;
-        break;
-      }
-      const Work w = sh.work[piece & 1];
-      if (w.token0 < 0) break;
+    auto wait_pair = [&] { return wait_warp(&sh.pair_full[it % kStages], (it / kStages) & 1, err); };
+    auto issue_s = [&](int i) {  // S_i = Q_i K^T
       tc_fence_after();
-      const int steps = max(w.count[0], w.count[1]);
-      auto wait_tile = [&](int index) {
-        return __all_sync(0xffffffffu, mbar_wait(&sh.kv_full[index % kStages], (index / kStages) & 1, err));
-      };
-      auto issue_s = [&](int i, int index) {  // S_i = Q_i K^T
-        const uint32_t qa = smem_addr(s_q) + i * kTile, ka = smem_addr(ring) + (index % kStages) * kTile;
+      if (elect_one()) {
+        const uint32_t qd = q_desc + i * (kTile >> 4), kd = k_desc + (it % kStages) * (2 * kTile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kHalf;
-          mma_smem(tmem + i * kBN, desc_kmajor(qa + off) + 2 * (kk & 3), desc_kmajor(ka + off) + 2 * (kk & 3), idesc_s,
-                   kk > 0 ? 1u : 0u);
+        for (uint32_t kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kHalf >> 4) + 2 * (kk & 3);  // 64-column half, 32 bytes per 16 columns
+          mma_smem(kTmem + i * kBN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
         }
         mma_commit(&sh.s_full[i]);
-      };
-      auto issue_o = [&](int i, int index, bool first) {  // O_i (+)= P_i V
-        const uint32_t va = smem_addr(ring) + (index % kStages) * kTile;
+      }
+      __syncwarp();
+    };
+    auto issue_o = [&](int i, bool first, int half) {  // O_i (+)= P_i V over 64 keys
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t vd = v_desc + (it % kStages) * (2 * kTile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk)
-          mma_tmem(tmem + 256 + i * kBN, tmem + i * kBN + kk * 8, desc_mnmajor(va + kk * 16 * 128), idesc_o,
+        for (uint32_t kk = half * 4; kk < half * 4 + 4; ++kk)
+          mma_tmem(kTmem + 256 + i * kBN, kTmem + i * kBN + kk * 8, vd + kk * (16 * 128 >> 4), idesc_o,
                    (!first || kk > 0) ? 1u : 0u);
-      };
-      if (!wait_tile(it)) {
+      }
+      __syncwarp();
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) mma_commit(bar);
+      __syncwarp();
+    };
+    bool ok = true;
+    for (int piece = 0; ok && !*abort_flag; ++piece) {
+      if (!wait_warp(&sh.q_full, piece & 1, err)) {
         ok = false;
         break;
       }
-      tc_fence_after();
-      if (lane == 0) {
-        for (int i = 0; i < 2; ++i)
-          if (w.count[i] > 0) issue_s(i, it);
-        mma_commit(&sh.kv_empty[it % kStages]);
-        if (steps == 1) mma_commit(&sh.q_empty);
+      const int token0 = sh.work[piece & 1].token0, count0 = sh.work[piece & 1].count[0],
+                count1 = sh.work[piece & 1].count[1], left = sh.work[piece & 1].keys - sh.work[piece & 1].tile0 * kBN;
+      if (token0 < 0) break;
+      const int count[2] = {static_cast<int>(__reduce_max_sync(0xffffffffu, count0)),
+                            static_cast<int>(__reduce_max_sync(0xffffffffu, count1))};
+      const int steps = max(count[0], count[1]);
+      if (!wait_pair()) {
+        ok = false;
+        break;
       }
-      __syncwarp();
-      for (int step = 0; step < steps && ok; ++step) {
-        const int v_index = it + 2 * step + 1, k_index = it + 2 * step + 2;
-        if (!wait_tile(v_index)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (count[i] > 0) issue_s(i);
+      commit(&sh.pair_empty[it % kStages]);
+      if (steps == 1) commit(&sh.q_empty);
+      ++it;
+      for (int step = 0; step < steps; ++step, ++it) {
+        if (!wait_pair()) {
           ok = false;
           break;
         }
-        const int valid = w.keys - (w.tile0 + step) * kBN;
+        const int valid = left - step * kBN;
         if (valid < kBN) {  // values past the block's keys: zeros, whatever is there
-          const uint32_t va = smem_addr(ring) + (v_index % kStages) * kTile;
+          const uint32_t va = smem_addr(ring) + (it % kStages) * 2 * kTile;
           for (int r = max(valid, 0) + (lane >> 3); r < kBN; r += 4)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -587,56 +679,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
-        for (int i = 0; i < 2 && ok; ++i) {
-          if (step < w.count[i]) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh.p_full[i], p_seen[i] & 1, err)) ||
-                (step == 0 && !__all_sync(0xffffffffu, mbar_wait(&sh.o_empty[i], (o_seen[i] & 1) ^ 1, err)))) {
-              ok = false;
-              break;
-            }
-            ++p_seen[i];
-            tc_fence_after();
-            if (lane == 0) {
-              issue_o(i, v_index, step == 0);
-              if (step + 1 == w.count[i]) mma_commit(&sh.o_full[i]);
-            }
-            __syncwarp();
-          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (step >= count[i]) continue;
+          if (step == 0) ok = wait_warp(&sh.o_empty[i], (o_seen[i]++ & 1) ^ 1, err);
+          ok = ok && wait_warp(&sh.p_full[i][0], p_seen[i] & 1, err);
+          if (!ok) break;
+          issue_o(i, step == 0, 0);
+          ok = wait_warp(&sh.p_full[i][1], p_seen[i]++ & 1, err);
+          if (!ok) break;
+          issue_o(i, step == 0, 1);
           // The next scores overwrite this tile's P: one thread's MMAs run in the order of their issue.
-          if (step + 1 < w.count[i]) {
-            if (i == 0 || w.count[0] <= step + 1) {
-              if (!wait_tile(k_index)) {
-                ok = false;
-                break;
-              }
-            }
-            tc_fence_after();
-            if (lane == 0) issue_s(i, k_index);
-            __syncwarp();
-          }
+          if (step + 1 < count[i]) issue_s(i);
+          else commit(&sh.o_full[i]);
         }
-        if (ok && lane == 0) {
-          mma_commit(&sh.kv_empty[v_index % kStages]);
-          if (step + 1 < steps) mma_commit(&sh.kv_empty[k_index % kStages]);
-          if (step + 2 == steps) mma_commit(&sh.q_empty);
-        }
-        __syncwarp();
+        if (!ok) break;
+        commit(&sh.pair_empty[it % kStages]);
+        if (step + 2 == steps) commit(&sh.q_empty);
       }
-      it += 2 * steps;
-      for (int i = 0; i < 2; ++i)
-        if (w.count[i] > 0) ++o_seen[i];
     }
     if (!ok) *abort_flag = 1;
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax, one row per thread
     const int i = warp >> 2;                                  // query tile
     const int r = (warp & 3) * 32 + lane;                     // row of it
     const int place = r / group, head = r - place * group;    // token and query head of the row
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lanes + i * kBN, t_o = tmem + lanes + 256 + i * kBN;
+    const uint32_t t_s = kTmem + lanes + i * kBN, t_o = kTmem + lanes + 256 + i * kBN;
     uint32_t s_seen = 0, o_seen = 0;
     bool ok = true;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, err)); };
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return wait_warp(bar, parity, err); };
     for (int piece = 0; ok && !*abort_flag; ++piece) {
       if (!wait_all(&sh.q_full, piece & 1)) {
         ok = false;
@@ -652,6 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int limit = 0;  // keys the row sees
       if (real) limit = kShared ? min(c.length(w.token0 + token), a.shared_keys) : max(0, w.position0 + token + 1);
       float m = -INFINITY, l = 0.f;
+      bool odd = false;  // scores that are infinite or not a number
       for (int step = 0; step < count && ok; ++step) {
         if (!wait_all(&sh.s_full[i], s_seen & 1)) {
           ok = false;
@@ -672,8 +747,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < kBN; ++e) t4[e & 3] = fmaxf(t4[e & 3], __uint_as_float(x[e]));
-        const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+        for (int e = 0; e < kBN / 2; ++e)
+          t4[e & 3] = max3(t4[e & 3], __uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        const float top = max3(max3(t4[0], t4[1], t4[2]), t4[3], t4[3]);
+        odd = odd || !(top < INFINITY);
         const bool moves = top > m + kSlack || (m == -INFINITY && top > m);
         const float next = moves ? top : m;
         const float base = next == -INFINITY ? 0.f : next * kScaleLog2;
@@ -693,24 +770,33 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         m = next;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = pair(kScaleLog2, kScaleLog2), base2 = pair(-base, -base);
+        uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           uint32_t packed[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float p0 = exp2_approx(__uint_as_float(x[b * 64 + 2 * e]) * kScaleLog2 - base);
-            const float p1 = exp2_approx(__uint_as_float(x[b * 64 + 2 * e + 1]) * kScaleLog2 - base);
-            sum[(2 * e) & 3] += p0;
-            sum[(2 * e + 1) & 3] += p1;
+            const uint64_t y = fma2(pair(__uint_as_float(x[b * 64 + 2 * e]), __uint_as_float(x[b * 64 + 2 * e + 1])), scale2, base2);
+            float p0, p1;
+            if ((e & 3) < kByCubic) {
+              exp2_pair(y, &p0, &p1);
+            } else {
+              unpair(y, &p0, &p1);
+              p0 = exp2_approx(p0);
+              p1 = exp2_approx(p1);
+            }
+            sum2[e & 1] = add2(sum2[e & 1], pair(p0, p1));
             packed[e] = pack_bf16x2(p0, p1);
           }
           tmem_st32(t_s + b * 32, packed);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          mbar_arrive(&sh.p_full[i][b]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tc_fence_before();
-        mbar_arrive(&sh.p_full[i]);
+        float s0, s1;
+        unpair(add2(sum2[0], sum2[1]), &s0, &s1);
+        l += s0 + s1;
       }
       if (!ok) break;
       if (count > 0 && !wait_all(&sh.o_full[i], o_seen & 1)) {
@@ -722,7 +808,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* rec = w.record >= 0 ? a.records + (static_cast<int64_t>(w.record) * 2 * kBM + i * kBM + r) * kRecord
                    : kShared    ? a.whole + out_row * kRecord
                                 : nullptr;
-      const float inv = limit > 0 ? 1.f / l : 0.f;
+      const bool sees = limit > w.tile0 * kBN;  // a key of this piece; else its weights are none, whatever they met
+      const float inv = rec ? 1.f : 1.f / l;
       bool finite = true;
       if (count > 0) {
 #pragma unroll
@@ -734,7 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float f[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            f[e] = l > 0.f || l != l ? __uint_as_float(o[e]) * (rec ? 1.f : inv) : 0.f;
+            f[e] = sees ? __uint_as_float(o[e]) * inv : 0.f;
             finite = finite && fabsf(f[e]) <= 3.4e38f;
           }
           if (rec) {
@@ -754,10 +841,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (rec && real) {
         rec[128] = m;
-        rec[129] = l;
+        rec[129] = sees ? l : 0.f;
       }
       // rows with something not finite: again, key by key
-      unsigned again = __ballot_sync(0xffffffffu, real && limit > w.tile0 * kBN && count > 0 && !(finite && l > 0.f));
+      unsigned again = __ballot_sync(0xffffffffu, real && sees && count > 0 && (odd || !finite));
       __syncwarp();
       while (again) {
         const int from = __ffs(again) - 1;
@@ -787,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(kTmem), "r"(kTmemCols));
   }
 }
 
