@@ -38,9 +38,11 @@ int paged_cache(const char* name, const void* k_pages, const void* v_pages, cons
   if (tokens < 0 || sequences < 0 || num_pages < 1 || max_pages < 1)
     return fail(IPE_ERR_ARGUMENT, "%s: bad sizes (%lld rows, %d sequences, %lld pages, %d per sequence)", name,
                 static_cast<long long>(tokens), sequences, static_cast<long long>(num_pages), max_pages);
-  // positions, cache rows and (token, head) rows are 32-bit numbers in the kernels; their byte offsets are 64-bit
+  // positions, cache rows, (token, head) rows and units of 64 keys are 32-bit numbers in the kernels; their
+  // byte offsets are 64-bit
   if (tokens * q_heads > INT32_MAX || num_pages > INT32_MAX / (static_cast<int64_t>(kv_heads) * page_size) ||
-      max_pages > (1 << 27) / page_size || sequences > (1 << 24))
+      max_pages > (1 << 27) / page_size || sequences > (1 << 24) ||
+      static_cast<int64_t>(sequences) * kv_heads > INT32_MAX / (static_cast<int64_t>(max_pages) * page_size / 64 + 1))
     return fail(IPE_ERR_UNSUPPORTED, "%s: sizes past the kernels' 32-bit row numbers", name);
   if (tokens == 0 || sequences == 0) return IPE_OK;
   if (!k_pages || !v_pages || !page_table || !lengths) return fail(IPE_ERR_ARGUMENT, "%s: null pointer", name);

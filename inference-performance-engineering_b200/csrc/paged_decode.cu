@@ -29,6 +29,7 @@ constexpr int kStages = 3;               // units in flight per CTA
 constexpr int kStageBytes = 2 * 16 * 256;  // one warp's keys and values of a unit
 constexpr int kCtasPerSm = 2;
 constexpr int kHeads = 8;                // columns of the products
+constexpr int kNothing = -2;             // an item without keys
 constexpr int kMergeStride = 132;        // floats; spreads a warp's 4 head pairs over the banks
 constexpr size_t kSmem = static_cast<size_t>(kStages) * kWarps * kStageBytes +
                          static_cast<size_t>(kWarps) * kHeads * kMergeStride * sizeof(float);
@@ -40,7 +41,7 @@ struct DecodeArgs {
   const bf16* v;
   bf16* out;
   float* records;    // [grid][2][G][kRecord]
-  int64_t* offsets;  // [sequences + 1]: units of one KV head before each sequence
+  int2* items;       // [sequences][kv_heads]: item_parts
   float* whole;      // null, or where rows that are not in parts go: [sequences][q_heads][kRecord], not to out
   int first;         // keys before this one are left out
   int q_heads;
@@ -74,7 +75,7 @@ struct Cursor {
 
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(const DecodeArgs a) {
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t warp_units[kWarps];
+  __shared__ int warp_units[kWarps];
   __shared__ Cursor start;
   __shared__ float stats[kWarps][kHeads][2];
   float* merge = reinterpret_cast<float*>(smem + static_cast<size_t>(kStages) * kWarps * kStageBytes);
@@ -86,50 +87,48 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   // ------------------------------------------------------------------ this CTA's run of units
   const int per = (c.sequences + kThreads - 1) / kThreads;
   const int s_lo = min(c.sequences, static_cast<int>(threadIdx.x) * per), s_hi = min(c.sequences, s_lo + per);
-  int64_t mine = 0;
+  int mine = 0;
   for (int s = s_lo; s < s_hi; ++s) mine += units_of(keys_of(a, s));
-  int64_t scan = mine;
+  int scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, scan, o);
+    const int up = __shfl_up_sync(0xffffffffu, scan, o);
     if (lane >= o) scan += up;
   }
   if (lane == 31) warp_units[warp] = scan;
   __syncthreads();
-  int64_t before = scan - mine, total = 0;
+  int before = scan - mine, total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += warp_units[w];
     total += warp_units[w];
   }
-  const int64_t units = total * c.kv_heads;
-  const int runs = runs_of(units, gridDim.x);
-  const int64_t u0 = run_start(units, blockIdx.x, runs), u1 = run_start(units, blockIdx.x + 1, runs);
+  const Deal deal(total * c.kv_heads, gridDim.x);
+  const int u0 = deal.start(blockIdx.x), count = deal.start(blockIdx.x + 1) - u0;
   for (int s = s_lo; s < s_hi; ++s) {
     const int keys = keys_of(a, s), n = units_of(keys);
-    if (blockIdx.x == 0) a.offsets[s] = before;
     if (n > 0 && u0 >= before * c.kv_heads && u0 < (before + n) * c.kv_heads) {
-      const int r = static_cast<int>(u0 - before * c.kv_heads);
+      const int r = u0 - before * c.kv_heads;
       start = Cursor{s, r / n, r % n, n, keys};
     }
     if (n == 0 && !a.whole && s % gridDim.x == blockIdx.x) {  // no keys: zeros
       uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(s) * a.q_heads * 128);
       for (int i = 0; i < a.q_heads * 16; ++i) row[i] = make_uint4(0, 0, 0, 0);
     }
+    if (n == 0 && s % gridDim.x == blockIdx.x)
+      for (int h = 0; h < c.kv_heads; ++h) a.items[static_cast<int64_t>(s) * c.kv_heads + h] = make_int2(kNothing, 0);
     before += n;
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[c.sequences] = total;
   __syncthreads();
-  if (blockIdx.x >= runs) {
+  if (static_cast<int>(blockIdx.x) >= deal.runs) {
     if (a.whole) pdl_wait();
     return;
   }
-  const int64_t count = u1 - u0;
 
   // ------------------------------------------------------------------ loads
   const uint32_t ring = smem_addr(smem) + warp * kStageBytes;  // stage i at + i * kWarps * kStageBytes
   Cursor ahead = start;
-  int64_t issued = 0;
+  int issued = 0;
   int page = 0;  // of `ahead`
   auto look_up = [&] {
     const int key0 = ahead.unit * kUnit + warp * 16;
@@ -172,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const int frow = (lane & 7) + ((lane >> 3) & 1) * 8, fcol = lane >> 4;  // K fragments
   const int trow = (lane & 7) + (lane >> 4) * 8, tcol = (lane >> 3) & 1;  // V fragments, transposed
   int stage = 0;
-  for (int64_t u = 0; u < count; ++u) {
+  for (int u = 0; u < count; ++u) {
     issue(stage == 0 ? kStages - 1 : stage - 1);
     if (fresh) {
       fresh = false;
@@ -255,6 +254,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       const bool whole = whole_start && at.unit + 1 == at.units;
       const int slot = first_piece ? 0 : 1;
       first_piece = false;
+      if (whole_start && threadIdx.x == 0)
+        a.items[static_cast<int64_t>(at.s) * c.kv_heads + at.h] =
+            item_parts(deal, u0 + u - at.unit, at.units, blockIdx.x);
       for (int g = 0; g < group; ++g) {
         float top = -INFINITY;
 #pragma unroll
@@ -290,57 +292,50 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
 }
 
 // The parts of a row, none where the sequence has no keys or the row is whole.
-__device__ __forceinline__ Parts decode_parts(const DecodeArgs& a, int ctas, int s, int head) {
-  const PagedCache& c = a.c;
-  const int group = a.q_heads / c.kv_heads;
+__device__ __forceinline__ Parts decode_parts(const DecodeArgs& a, int s, int head) {
+  const int group = a.q_heads / a.c.kv_heads;
+  const int2 item = __ldcg(a.items + static_cast<int64_t>(s) * a.c.kv_heads + head / group);
   Parts p;
-  p.none();
-  const int64_t from = __ldcg(a.offsets + s), n = __ldcg(a.offsets + s + 1) - from;
-  if (n == 0) return p;
-  p.base = a.records;
-  p.rows = group;
-  p.row = head % group;
-  p.find(from * c.kv_heads + head / group * n, n, __ldcg(a.offsets + c.sequences) * c.kv_heads, ctas);
-  if (p.lo == p.hi) {
-    if (a.whole) p.single(a.whole + (static_cast<int64_t>(s) * a.q_heads + head) * kRecord);
-    else p.none();
-  }
+  p.rows(a.records, head % group, group, item);
+  if (item.x < 0) p.none();
+  if (item.x == kWhole && a.whole) p.single(a.whole + (static_cast<int64_t>(s) * a.q_heads + head) * kRecord);
   return p;
 }
 
 // One warp per (sequence, query head) in parts.
-__global__ void __launch_bounds__(kThreads) paged_decode_merge_kernel(const DecodeArgs a, int ctas) {
+__global__ void __launch_bounds__(kThreads) paged_decode_merge_kernel(const DecodeArgs a) {
+  const int row = static_cast<int>(blockIdx.x * kWarps + (threadIdx.x >> 5));
+  if (row >= a.c.sequences * a.q_heads) return;
+  const int s = row / a.q_heads, head = row - s * a.q_heads;
   pdl_wait();
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  if (row >= static_cast<int64_t>(a.c.sequences) * a.q_heads) return;
-  const Parts parts[1] = {decode_parts(a, ctas, static_cast<int>(row / a.q_heads), static_cast<int>(row % a.q_heads))};
-  if (parts[0].hi >= parts[0].lo) join_parts(parts, a.out + row * 128);
+  const Parts parts[1] = {decode_parts(a, s, head)};
+  if (parts[0].count() > 0) join_parts(parts, a.out + static_cast<int64_t>(row) * 128);
 }
 
 // One warp per (sequence, query head): the parts of the shared keys and those of the sequence's own.
-__global__ void __launch_bounds__(kThreads) shared_prefix_merge_kernel(const DecodeArgs a, int ctas, const SharedKeys shared) {
-  pdl_wait();
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5;
-  if (row >= static_cast<int64_t>(a.c.sequences) * a.q_heads) return;
-  const int s = static_cast<int>(row / a.q_heads), head = static_cast<int>(row % a.q_heads), lane = threadIdx.x & 31;
-  if (a.c.length(s) == 0) {
-    *reinterpret_cast<uint2*>(a.out + row * 128 + lane * 4) = make_uint2(0u, 0u);
-    return;
-  }
+__global__ void __launch_bounds__(kThreads) shared_prefix_merge_kernel(const DecodeArgs a, const SharedKeys shared) {
+  const int row = static_cast<int>(blockIdx.x * kWarps + (threadIdx.x >> 5)), lane = threadIdx.x & 31;
+  if (row >= a.c.sequences * a.q_heads) return;
+  const int s = row / a.q_heads, head = row - s * a.q_heads;
   const int group = a.q_heads / a.c.kv_heads, per_block = 2 * shared.per_tile;
   const int block = s / per_block, in_block = s % per_block, tile = in_block / shared.per_tile;
+  bf16* out = a.out + static_cast<int64_t>(row) * 128;
+  const bool empty = a.c.length(s) == 0;
+  pdl_wait();
+  if (empty) {
+    *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(0u, 0u);
+    return;
+  }
+  const int2 item = __ldcg(shared.items + static_cast<int64_t>(block) * a.c.kv_heads + head / group);
   Parts parts[2];
-  parts[0].base = shared.records;
-  parts[0].rows = 256;
-  parts[0].row = tile * 128 + (in_block - tile * shared.per_tile) * group + head % group;
-  parts[0].find((static_cast<int64_t>(block) * a.c.kv_heads + head / group) * shared.tiles, shared.tiles, shared.units,
-                shared.ctas);
-  if (parts[0].lo == parts[0].hi) parts[0].single(shared.whole + row * kRecord);
-  parts[1] = decode_parts(a, ctas, s, head);
-  join_parts(parts, a.out + row * 128);
+  parts[0].blocks(shared.records, tile * 128 + (in_block - tile * shared.per_tile) * group + head % group, item);
+  // whole (or what a kernel that gave up on a wait left)
+  if (item.x < 0 || item.y >= shared.ctas || item.y < item.x >> 1) parts[0].single(shared.whole + static_cast<int64_t>(row) * kRecord);
+  parts[1] = decode_parts(a, s, head);
+  join_parts(parts, out);
 }
 
-size_t offsets_bytes(int sequences) { return ((static_cast<size_t>(sequences) + 1) * sizeof(int64_t) + 255) / 256 * 256; }
+size_t items_bytes(int64_t items) { return (static_cast<size_t>(items) * sizeof(int2) + 255) / 256 * 256; }
 
 DecodeArgs decode_args(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out, int q_heads,
                        void* workspace) {
@@ -350,8 +345,9 @@ DecodeArgs decode_args(const PagedCache& c, const void* q, const void* k_pages, 
   a.k = static_cast<const bf16*>(k_pages);
   a.v = static_cast<const bf16*>(v_pages);
   a.out = static_cast<bf16*>(out);
-  a.offsets = static_cast<int64_t*>(workspace);
-  a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + offsets_bytes(c.sequences));
+  a.items = static_cast<int2*>(workspace);
+  a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
+                                       items_bytes(static_cast<int64_t>(c.sequences) * c.kv_heads));
   a.q_heads = q_heads;
   return a;
 }
@@ -369,7 +365,7 @@ dim3 merge_grid(const PagedCache& c, int q_heads) {
 }  // namespace
 
 size_t paged_decode_workspace_bytes(int sequences, int q_heads, int kv_heads) {
-  return offsets_bytes(sequences) + static_cast<size_t>(kCtasPerSm * sm_count()) * 2 * (q_heads / kv_heads) * kRecord * sizeof(float);
+  return items_bytes(static_cast<int64_t>(sequences) * kv_heads) + static_cast<size_t>(kCtasPerSm * sm_count()) * 2 * (q_heads / kv_heads) * kRecord * sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
@@ -382,13 +378,14 @@ cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* 
   paged_decode_kernel<<<grid, kThreads, kSmem, stream>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess || (c.max_pages << c.page_shift) <= kUnit) return e;  // one unit per item: nothing to merge
-  return launch_pdl(paged_decode_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a, grid);
+  return launch_pdl(paged_decode_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a);
 }
 
 size_t shared_prefix_workspace_bytes(const PagedCache& c, int q_heads) {
   const size_t rows = static_cast<size_t>(c.sequences) * q_heads * kRecord * sizeof(float);
-  return 2 * rows + static_cast<size_t>(shared_keys_plan(c, q_heads).ctas) * 2 * 256 * kRecord * sizeof(float) +
-         paged_decode_workspace_bytes(c.sequences, q_heads, c.kv_heads);
+  const SharedKeys plan = shared_keys_plan(c, q_heads);
+  return paged_decode_workspace_bytes(c.sequences, q_heads, c.kv_heads) + items_bytes(plan.items_count) + 2 * rows +
+         static_cast<size_t>(plan.ctas) * 2 * kBlockRecord * sizeof(float);
 }
 
 cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
@@ -400,8 +397,9 @@ cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void*
   const size_t rows = static_cast<size_t>(c.sequences) * q_heads * kRecord;
   SharedKeys shared = shared_keys_plan(c, q_heads);
   DecodeArgs a = decode_args(c, q, k_pages, v_pages, out, q_heads, workspace);
-  shared.whole = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) +
-                                          paged_decode_workspace_bytes(c.sequences, q_heads, c.kv_heads));
+  unsigned char* behind = static_cast<unsigned char*>(workspace) + paged_decode_workspace_bytes(c.sequences, q_heads, c.kv_heads);
+  shared.items = reinterpret_cast<int2*>(behind);
+  shared.whole = reinterpret_cast<float*>(behind + items_bytes(shared.items_count));
   a.whole = shared.whole + rows;
   shared.records = a.whole + rows;
   a.first = c.prefix_count << c.page_shift;
@@ -411,7 +409,7 @@ cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void*
   const int grid = decode_grid(c);
   e = launch_pdl(paged_decode_kernel, dim3(grid), dim3(kThreads), kSmem, stream, a);
   if (e != cudaSuccess) return e;
-  return launch_pdl(shared_prefix_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a, grid, shared);
+  return launch_pdl(shared_prefix_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a, shared);
 }
 
 }  // namespace ipe

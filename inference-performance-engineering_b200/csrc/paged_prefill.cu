@@ -62,9 +62,8 @@ struct Shared {
   uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
   uint32_t tmem;
   int abort;
-  int blocks;
-  int warp_sums[16];
   Work work[2];
+  alignas(16) uint4 stage[8][32 * 4];  // by softmax warp
   int low[kMaxListed + 1], high[kMaxListed + 1];
 };
 constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + 2 * kStages) * kTile + sizeof(Shared);
@@ -75,12 +74,14 @@ struct PrefillArgs {
   const bf16* k;
   const bf16* v;
   bf16* out;
-  float* records;  // [grid][2][256][kRecord] where the key tiles are dealt in runs, else null
-  int* lists;      // [2][kMaxListed + 1]: blocks before each sequence, key tiles before each block
+  float* records;  // [grid][2][kBlockRecord] where the key tiles are dealt in runs, else null
+  int2* items;     // in runs: [blocks][kv_heads], item_parts
+  int4* blocks;    // in runs: of each block token0, tokens, position0; before them, how many there are
   float* whole;    // shared keys: where rows that are not in parts go, [tokens][q_heads][kRecord]
   int tokens;
   int q_heads;
   int shared_keys;
+  int most_blocks;  // in runs: room for so many
 };
 
 // Shared-memory operands with the 128-byte swizzle, 8-row groups 1024 bytes apart. The upper words of
@@ -296,27 +297,26 @@ __device__ __forceinline__ Work make_work(const Span& x, int s, int b, int kv_he
   return w;
 }
 
-// exclusive prefix sums of x over the block's threads; the total in *total
-__device__ int block_scan(int x, int* warp_sums, int* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// exclusive prefix sums of x over the warp
+__device__ __forceinline__ int warp_scan(int x) {
   int scan = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += up;
+    if ((threadIdx.x & 31) >= o) scan += up;
   }
-  __syncthreads();
-  if (lane == 31) warp_sums[warp] = scan;
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const int n = warp_sums[w];
-    if (w < warp) before += n;
-    all += n;
+  return scan - x;
+}
+
+// the last index below n whose value is at most x, of an ascending list that starts with 0
+__device__ __forceinline__ int last_at_most(const int* list, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (list[mid] <= x) lo = mid;
+    else hi = mid;
   }
-  *total = all;
-  return before + scan - x;
+  return lo;
 }
 
 // kShared: the "new tokens" are one query token of each sequence, all on the pages of c.prefix_pages (a
@@ -363,76 +363,76 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
 
-  // ------------------------------------------------------------------ blocks
-  // In runs: sh.low = blocks before each sequence, sh.high = key tiles before each block. Otherwise
-  // sh.low .. sh.high: the sequence's blocks as numbers that grow with their keys (block 0 of a sequence
-  // on a context starts at the context's length in blocks).
-  const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
-  int blocks = kShared ? (a.tokens + per_block - 1) / per_block : 0;
-  for (int base = 0; !kShared && base < c.sequences; base += kThreads) {
-    const int s = base + threadIdx.x;
-    Span x{0, 0, 0};
-    if (s < c.sequences) x = span_of(c, s, a.tokens);
-    const int n = (x.tokens + per_block - 1) / per_block;
-    int all;
-    const int before = block_scan(n, sh.warp_sums, &all);
-    if (s < c.sequences && s < kMaxListed) {
-      const int first = max(0, x.length - x.tokens) / per_block;
-      sh.low[s] = in_runs ? min(blocks + before, kMaxListed) : first;
-      if (!in_runs) sh.high[s] = first + n;
-    }
-    blocks += all;
-  }
-  int tiles = kShared ? blocks * shared_tiles : 0;
-  if (!kShared && in_runs) {
-    blocks = min(blocks, kMaxListed);
-    const int listed = min(c.sequences, kMaxListed);
-    if (threadIdx.x == 0) sh.low[listed] = blocks;
-    __syncthreads();
-    for (int base = 0; base < blocks; base += kThreads) {
-      const int i = base + threadIdx.x;
-      int n = 0;
-      if (i < blocks) {
-        int lo = 0, hi = listed;  // the last sequence with low[s] <= i
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (sh.low[mid] <= i) lo = mid;
-          else hi = mid;
-        }
-        n = tiles_of(block_keys(span_of(c, lo, a.tokens), i - sh.low[lo], per_block));
-      }
-      int all;
-      const int before = block_scan(n, sh.warp_sums, &all);
-      if (i < blocks) sh.high[i] = tiles + before;
-      tiles += all;
-    }
-    if (threadIdx.x == 0) sh.high[blocks] = tiles;
-    __syncthreads();
-    if (blockIdx.x == 0) {
-      for (int i = threadIdx.x; i <= kMaxListed; i += kThreads) {
-        if (i <= listed) a.lists[i] = sh.low[i];
-        if (i <= blocks) a.lists[kMaxListed + 1 + i] = sh.high[i];
-      }
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (threadIdx.x == 0 && sh.tmem != kTmem) report(err, kErrShape);
-  const int64_t units = static_cast<int64_t>(tiles) * c.kv_heads;
-  const int runs = runs_of(units, gridDim.x);
-
   if (warp >= kLoadWarp) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ work list and loads
+    if (lane < 3)
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v))
+                   : "memory");
     const int ps = c.page_size(), subs = kBN >> c.page_shift;
-    const int64_t works = static_cast<int64_t>(blocks) * c.kv_heads;
-    int64_t unit = 0, unit_end = 0;  // in runs
-    if (in_runs && static_cast<int>(blockIdx.x) < runs) {
-      unit = run_start(units, blockIdx.x, runs);
-      unit_end = run_start(units, blockIdx.x + 1, runs);
+    // In runs: sh.low = blocks before each sequence, sh.high = key tiles before each block. Otherwise
+    // sh.low .. sh.high: the sequence's blocks as numbers that grow with their keys (block 0 of a sequence
+    // on a context starts at the context's length in blocks), `most` past the largest.
+    const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
+    int blocks = 0, tiles = 0, most = 0;
+    bool whole = false;
+    if (kShared) {
+      blocks = (a.tokens + per_block - 1) / per_block;
+      tiles = blocks * shared_tiles;
+    } else {
+      for (int base = 0; base < c.sequences; base += 32) {
+        const int s = base + lane;
+        Span x{0, 0, 0};
+        if (s < c.sequences) x = span_of(c, s, a.tokens);
+        const int n = (x.tokens + per_block - 1) / per_block, first = max(0, x.length - x.tokens) / per_block;
+        const int before = blocks + warp_scan(n);
+        if (s < kMaxListed) {
+          sh.low[s] = in_runs ? min(before, a.most_blocks) : first;
+          sh.high[s] = first + n;
+        }
+        if (n > 0) most = max(most, first + n);
+        blocks = __shfl_sync(0xffffffffu, before + n, 31);
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      __syncwarp();
     }
+    if (!kShared && in_runs) {
+      blocks = min(blocks, a.most_blocks);
+      if (blockIdx.x == 0 && lane == 0) a.blocks[-1].x = blocks;
+      int longest = 0;
+      for (int base = 0; base < blocks; base += 32) {
+        const int i = base + lane;
+        int n = 0;
+        if (i < blocks) {
+          const int s = last_at_most(sh.low, c.sequences, i);
+          n = tiles_of(block_keys(span_of(c, s, a.tokens), i - sh.low[s], per_block));
+        }
+        const int before = tiles + warp_scan(n);
+        if (i < blocks) sh.high[i] = before;
+        longest = max(longest, n);
+        tiles = __shfl_sync(0xffffffffu, before + n, 31);
+      }
+      // Whole blocks after all where the runs would save less than the records and their merge cost, which
+      // is the time of about 5 key tiles (9 us).
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      const int ctas = gridDim.x;
+      whole = longest * ((blocks * c.kv_heads + ctas - 1) / ctas) <= (tiles * c.kv_heads + ctas - 1) / ctas + 5;
+      if (whole) {
+        for (int i = lane; i < blocks; i += 32) sh.high[i] = i;  // a block is one unit
+        tiles = blocks;
+      }
+      if (lane == 0) sh.high[blocks] = tiles;
+      __syncwarp();
+    }
+    const int works = blocks * c.kv_heads;
+    const Deal deal(in_runs ? tiles * c.kv_heads : 0, gridDim.x);
+    int unit = deal.start(blockIdx.x);  // in runs
+    const int unit_end = deal.start(blockIdx.x + 1);
     const bool listed = c.sequences <= kMaxListed;
     auto range_of = [&](int s, int* low, int* high) {
       if (listed) {
@@ -455,13 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
       };
-      int most = 0;
-      for (int s = lane; s < c.sequences; s += 32) {
-        int low, high;
-        range_of(s, &low, &high);
-        most = max(most, high);
-      }
-      int lo = 0, hi = static_cast<int>(__reduce_max_sync(0xffffffffu, most));  // at_least(lo) > rank >= at_least(hi)
+      int lo = 0, hi = most;  // at_least(lo) > rank >= at_least(hi)
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (at_least(mid) > rank) lo = mid;
@@ -489,67 +483,41 @@ __global__ void __launch_bounds__(kThreads, 1)
     int slot = 0, piece = 0;
     uint32_t phase = 0, armed = 0;  // bit s: parity armed on pair_full[s]; bit 16 + s: armed at all
     bool ok = true;
-    for (int64_t round = 0; ok && !*abort_flag; ++round, ++piece) {
+    for (int round = 0; ok && !*abort_flag; ++round, ++piece) {
       Work w;
       if (in_runs) {
         if (unit >= unit_end) break;
-        int lo = 0, hi = blocks;  // the block of this unit: the last with high[i] * kv_heads <= unit
-        if (kShared) {
-          lo = static_cast<int>(unit / (static_cast<int64_t>(shared_tiles) * c.kv_heads));
-          hi = lo + 1;
-        }
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (static_cast<int64_t>(sh.high[mid]) * c.kv_heads <= unit) lo = mid;
-          else hi = mid;
-        }
-        const int block = lo, before = kShared ? block * shared_tiles : sh.high[block];
+        const int block = kShared ? unit / (shared_tiles * c.kv_heads) : last_at_most(sh.high, blocks, unit / c.kv_heads);
+        const int before = kShared ? block * shared_tiles : sh.high[block];
         const int n = kShared ? shared_tiles : sh.high[block + 1] - before;
-        const int r = static_cast<int>(unit - static_cast<int64_t>(before) * c.kv_heads);
-        const int tile0 = r % n, tile1 = static_cast<int>(min(static_cast<int64_t>(n), tile0 + unit_end - unit));
+        const int r = unit - before * c.kv_heads, kv_head = r / n;
+        const int tile0 = r - kv_head * n, tile1 = min(n, tile0 + unit_end - unit);
+        if (tile0 == 0 && lane == 0)
+          a.items[static_cast<int64_t>(block) * c.kv_heads + kv_head] = item_parts(deal, unit, n, blockIdx.x);
         if (kShared) {
           // every row sees up to all shared keys: as if the tokens stood behind them
-          w = make_work(Span{0, a.tokens, a.shared_keys + a.tokens}, 0, block, r / n, per_tile, tile0, tile1);
+          w = make_work(Span{0, a.tokens, a.shared_keys + a.tokens}, 0, block, kv_head, per_tile, tile0, tile1);
           w.keys = a.shared_keys;
 #pragma unroll
           for (int i = 0; i < 2; ++i) w.count[i] = w.tokens > i * per_tile ? tile1 - tile0 : 0;
         } else {
-          lo = 0;
-          hi = min(c.sequences, kMaxListed);
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (sh.low[mid] <= block) lo = mid;
-            else hi = mid;
-          }
-          w = make_work(span_of(c, lo, a.tokens), lo, block - sh.low[lo], r / n, per_tile, tile0, tile1);
+          const int s = last_at_most(sh.low, c.sequences, block);
+          w = make_work(span_of(c, s, a.tokens), s, block - sh.low[s], kv_head, per_tile, tile0, whole ? -1 : tile1);
+          if (tile0 == 0 && kv_head == 0 && lane == 0) a.blocks[block] = make_int4(w.token0, w.tokens, w.position0, 0);
         }
         if (tile0 > 0 || tile1 < n) w.record = static_cast<int>(blockIdx.x) * 2 + (round == 0 ? 0 : 1);
         unit += tile1 - tile0;
       } else {
-        const int64_t rank = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        if (round * static_cast<int64_t>(gridDim.x) >= works) break;
+        const int ctas = gridDim.x, turn = round * ctas;
+        const int rank = turn + ((round & 1) ? ctas - 1 - blockIdx.x : blockIdx.x);
+        if (turn >= works) break;
         if (rank >= works) {
           --piece;  // nothing this round; the next one is empty
           continue;
         }
         int s, b;
-        select(static_cast<int>(rank / c.kv_heads), &s, &b);
-        w = make_work(span_of(c, s, a.tokens), s, b, static_cast<int>(rank % c.kv_heads), per_tile, 0, -1);
-      }
-      if (!wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
-        ok = false;
-        break;
-      }
-      if (lane == 0) {
-        sh.work[piece & 1] = w;
-        const int rows = group * per_tile * 128;  // bytes of a query tile's half
-        const int n = w.tokens > per_tile ? 2 : 1;
-        mbar_expect_tx(&sh.q_full, 2 * rows * n);
-        for (int i = 0; i < n; ++i) {
-          const uint32_t dst = smem_addr(s_q) + i * kTile;
-          tma_load_3d(dst, &map_q, &sh.q_full, 0, w.kv_head * group, w.token0 + i * per_tile);
-          tma_load_3d(dst + kHalf, &map_q, &sh.q_full, 64, w.kv_head * group, w.token0 + i * per_tile);
-        }
+        select(rank / c.kv_heads, &s, &b);
+        w = make_work(span_of(c, s, a.tokens), s, b, rank % c.kv_heads, per_tile, 0, -1);
       }
       const int steps = max(w.count[0], w.count[1]);
       // This lane's page of a step's tile: its ID is loaded a step ahead and looked at when it is used.
@@ -578,6 +546,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_2d(dst + kTile + kHalf, &map_k, &sh.pair_full[slot], 64, row);
         }
         armed = (armed & ~(1u << slot)) | (phase << slot) | (1u << (16 + slot));
+        if (step == 0) {  // the block's queries, once the piece before is done with its own
+          if (!wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            sh.work[piece & 1] = w;
+            const int rows = group * per_tile * 128;  // bytes of a query tile's half
+            const int n = w.tokens > per_tile ? 2 : 1;
+            mbar_expect_tx(&sh.q_full, 2 * rows * n);
+            for (int i = 0; i < n; ++i) {
+              const uint32_t dst_q = smem_addr(s_q) + i * kTile;
+              tma_load_3d(dst_q, &map_q, &sh.q_full, 0, w.kv_head * group, w.token0 + i * per_tile);
+              tma_load_3d(dst_q + kHalf, &map_q, &sh.q_full, 64, w.kv_head * group, w.token0 + i * per_tile);
+            }
+          }
+          __syncwarp();
+        }
         if (++slot == kStages) {
           slot = 0;
           phase ^= 1;
@@ -805,46 +791,64 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const int64_t out_row = static_cast<int64_t>(w.token0 + token) * a.q_heads + w.kv_head * group + head;
-      float* rec = w.record >= 0 ? a.records + (static_cast<int64_t>(w.record) * 2 * kBM + i * kBM + r) * kRecord
-                   : kShared    ? a.whole + out_row * kRecord
-                                : nullptr;
+      // where the row goes unless to the output
+      const bool part = w.record >= 0;
+      const int record_row = i * kBM + r;
+      float* rec = part      ? a.records + static_cast<int64_t>(w.record) * kBlockRecord + record_row * 8
+                   : kShared ? a.whole + out_row * kRecord
+                             : nullptr;
+      const int at_m = part ? kBlockRows * 128 - record_row * 7 : 128, at_sum = part ? at_m + kBlockRows : 129;
       const bool sees = limit > w.tile0 * kBN;  // a key of this piece; else its weights are none, whatever they met
       const float inv = rec ? 1.f : 1.f / l;
-      bool finite = true;
+      float largest = 0.f;  // NaN if something is
       if (count > 0) {
-#pragma unroll
+        // Rows go out through shared memory, 64 bytes of 8 rows per store: 16 bytes of 32 rows each would
+        // take the L1 a cycle per row and store, 4000 for the two tiles.
+        const int out_rows = real ? static_cast<int>(out_row) : -1;
+        uint4* stage = sh.stage[warp];
+#pragma unroll 1
         for (int b = 0; b < kD / 32; ++b) {
           uint32_t o[32];
           tmem_ld32(t_o + b * 32, o);
           tmem_ld_wait(o);
-          if (!real) continue;
           float f[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            f[e] = sees ? __uint_as_float(o[e]) * inv : 0.f;
-            finite = finite && fabsf(f[e]) <= 3.4e38f;
-          }
-          if (rec) {
+          for (int e = 0; e < 32; ++e) f[e] = sees ? __uint_as_float(o[e]) * inv : 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              *reinterpret_cast<float4*>(rec + b * 32 + 4 * e) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          for (int e = 0; e < 16; ++e) largest = max3(largest, fabsf(f[2 * e]), fabsf(f[2 * e + 1]));
+          if (rec) {
+            if (real) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<float4*>(rec + (part ? block_vector(b * 8 + e) : (b * 8 + e) * 4)) =
+                    make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+            }
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(a.out + out_row * 128 + b * 32 + 8 * e) = pack8(f + 8 * e);
+            for (int e = 0; e < 4; ++e) stage[lane * 4 + (e ^ (lane >> 1 & 3))] = pack8(f + 8 * e);
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int from = q * 8 + (lane >> 2), row = __shfl_sync(0xffffffffu, out_rows, from);
+              if (row >= 0)
+                *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(row) * 128 + b * 32 + (lane & 3) * 8) =
+                    stage[from * 4 + ((lane & 3) ^ (from >> 1 & 3))];
+            }
+            __syncwarp();
           }
         }
         tc_fence_before();
         mbar_arrive(&sh.o_empty[i]);
         ++o_seen;
       } else if (rec && real) {
-        for (int e = 0; e < kD; e += 4) *reinterpret_cast<float4*>(rec + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int e = 0; e < kD / 4; ++e) *reinterpret_cast<float4*>(rec + block_vector(e)) = make_float4(0.f, 0.f, 0.f, 0.f);
       }
       if (rec && real) {
-        rec[128] = m;
-        rec[129] = sees ? l : 0.f;
+        rec[at_m] = m;
+        rec[at_sum] = sees ? l : 0.f;
       }
       // rows with something not finite: again, key by key
-      unsigned again = __ballot_sync(0xffffffffu, real && sees && count > 0 && (odd || !finite));
+      unsigned again = __ballot_sync(0xffffffffu, real && sees && count > 0 && (odd || !(largest <= 3.4e38f)));
       __syncwarp();
       while (again) {
         const int from = __ffs(again) - 1;
@@ -855,10 +859,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         attend_row(c, a.q + row * 128, a.k, a.v, w.sequence, w.kv_head, first, min(keys, first + count * kBN), o, &top, &sum);
         if (rec) {
           float* at = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(rec), from));
-          *reinterpret_cast<float4*>(at + lane * 4) = make_float4(o[0], o[1], o[2], o[3]);
-          if (lane == 0) {
-            at[128] = top;
-            at[129] = sum;
+          *reinterpret_cast<float4*>(at + (part ? block_vector(lane) : lane * 4)) = make_float4(o[0], o[1], o[2], o[3]);
+          if (lane == from) {
+            rec[at_m] = top;
+            rec[at_sum] = sum;
           }
         } else {
           const float s = 1.f / sum;
@@ -878,41 +882,31 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// One warp per (token, query head) whose block's key tiles lie in more than one run: merges the records.
-__global__ void __launch_bounds__(128) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
+// The blocks whose key tiles lie in more than one run: a CTA per (block, KV head, 16 rows), a warp per row at
+// a time.
+constexpr int kMergeRows = 16;
+__global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
+  const int block = blockIdx.x / a.c.kv_heads, kv_head = blockIdx.x - block * a.c.kv_heads;
+  const int group = a.q_heads / a.c.kv_heads, per_tile = kBM / group;
   pdl_wait();
-  const int64_t warp = (static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x) >> 5;
-  const PagedCache& c = a.c;
-  if (warp >= static_cast<int64_t>(a.tokens) * a.q_heads) return;
-  const int lane = threadIdx.x & 31;
-  const int t = static_cast<int>(warp / a.q_heads), head = static_cast<int>(warp % a.q_heads);
-  const int s = find_sequence(c.cu_tokens, c.sequences, t);
-  if (s < 0) return;
-  const Span x = span_of(c, s, a.tokens);
-  if (t < x.begin || t >= x.begin + x.tokens || s >= kMaxListed) return;
-  const int group = a.q_heads / c.kv_heads, per_tile = kBM / group, per_block = 2 * per_tile;
-  const int listed = min(c.sequences, kMaxListed);
-  const int blocks = __ldcg(a.lists + listed);
-  const int place = t - x.begin, block = __ldcg(a.lists + s) + place / per_block;
-  if (block >= blocks) return;
-  const int* before = a.lists + kMaxListed + 1;
-  const int tile0 = __ldcg(before + block), n = __ldcg(before + block + 1) - tile0;
-  const int64_t units = static_cast<int64_t>(__ldcg(before + blocks)) * c.kv_heads;
-  Parts parts[1];
-  parts[0].base = a.records;
-  parts[0].rows = 2 * kBM;
-  const int in_block = place % per_block, tile = in_block / per_tile;
-  parts[0].row = tile * kBM + (in_block - tile * per_tile) * group + head % group;
-  parts[0].find(static_cast<int64_t>(tile0) * c.kv_heads + static_cast<int64_t>(head / group) * n, n, units, ctas);
-  if (parts[0].lo == parts[0].hi) return;  // whole, already written
-  bf16* row = a.out + warp * 128;
-  if (x.length - x.tokens + place < 0)  // no position: no keys
-    *reinterpret_cast<uint2*>(row + lane * 4) = make_uint2(0u, 0u);
-  else
-    join_parts(parts, row);
+  if (block >= min(__ldcg(&a.blocks[-1].x), a.most_blocks)) return;
+  const int2 item = __ldcg(a.items + blockIdx.x);
+  // whole, already written; or what a kernel that gave up on a wait left
+  if (item.x < 0 || item.y >= ctas || item.y < item.x >> 1) return;
+  const int4 b = __ldcg(a.blocks + block);
+  for (int k = threadIdx.x >> 5; k < kMergeRows; k += 8) {
+    const int r = blockIdx.y * kMergeRows + k, tile = r / kBM, in_tile = r - tile * kBM;
+    const int place = in_tile / group, token = tile * per_tile + place;
+    if (place >= per_tile || token >= b.y || b.x < 0 || b.x + token >= a.tokens) continue;
+    bf16* row = a.out + (static_cast<int64_t>(b.x + token) * a.q_heads + kv_head * group + in_tile - place * group) * 128;
+    Parts parts[1];
+    parts[0].blocks(a.records, r, item);
+    if (b.z + token < 0)  // no position: no keys
+      *reinterpret_cast<uint2*>(row + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
+    else
+      join_parts(parts, row);
+  }
 }
-
-constexpr size_t kListBytes = (2 * (kMaxListed + 1) * sizeof(int) + 255) / 256 * 256;
 
 // most blocks that `tokens` new tokens of `sequences` sequences make
 int64_t most_blocks(int64_t tokens, int sequences, int group) {
@@ -926,11 +920,16 @@ bool deal_in_runs(int64_t tokens, int sequences, int q_heads, int kv_heads) {
   return blocks <= kMaxListed && sequences <= kMaxListed && blocks * kv_heads < 2 * sm_count();
 }
 
+size_t list_bytes(size_t blocks, int kv_heads) {
+  return (sizeof(int4) + blocks * (sizeof(int4) + kv_heads * sizeof(int2)) + 255) / 256 * 256;
+}
+
 }  // namespace
 
 size_t paged_prefill_workspace_bytes(int64_t tokens, int sequences, int q_heads, int kv_heads) {
   if (!deal_in_runs(tokens, sequences, q_heads, kv_heads)) return 0;
-  return kListBytes + static_cast<size_t>(sm_count()) * 2 * 2 * kBM * kRecord * sizeof(float);
+  const size_t blocks = static_cast<size_t>(most_blocks(tokens, sequences, q_heads / kv_heads));
+  return list_bytes(blocks, kv_heads) + static_cast<size_t>(sm_count()) * 2 * kBlockRecord * sizeof(float);
 }
 
 namespace {
@@ -976,18 +975,20 @@ cudaError_t launch_paged_prefill(const PagedCache& c, const void* q, const void*
   if (e != cudaSuccess) return e;
   a.out = static_cast<bf16*>(out);
   const bool in_runs = deal_in_runs(tokens, c.sequences, q_heads, c.kv_heads);
-  int64_t grid = most_blocks(tokens, c.sequences, q_heads / c.kv_heads) * c.kv_heads;
+  const int64_t blocks = most_blocks(tokens, c.sequences, q_heads / c.kv_heads);
+  int64_t grid = blocks * c.kv_heads;
   if (in_runs) {
-    a.lists = static_cast<int*>(workspace);
-    a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kListBytes);
+    a.blocks = static_cast<int4*>(workspace) + 1;
+    a.most_blocks = static_cast<int>(blocks);
+    a.items = reinterpret_cast<int2*>(a.blocks + blocks);
+    a.records = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + list_bytes(blocks, c.kv_heads));
     grid *= ((static_cast<int64_t>(c.max_pages) << c.page_shift) + kBN - 1) / kBN;
   }
   grid = std::min<int64_t>(grid, sm_count());
   e = launch<false>(grid, maps, a, stream);
   if (e != cudaSuccess || !in_runs) return e;
-  const int64_t warps = tokens * q_heads;
-  return launch_pdl(paged_prefill_merge_kernel, dim3(static_cast<unsigned>((warps + 3) / 4)), dim3(128), 0, stream, a,
-                    static_cast<int>(grid));
+  return launch_pdl(paged_prefill_merge_kernel, dim3(static_cast<unsigned>(blocks * c.kv_heads), 2 * kBM / kMergeRows),
+                    dim3(256), 0, stream, a, static_cast<int>(grid));
 }
 
 SharedKeys shared_keys_plan(const PagedCache& c, int q_heads) {
@@ -995,7 +996,8 @@ SharedKeys shared_keys_plan(const PagedCache& c, int q_heads) {
   p.per_tile = kBM / (q_heads / c.kv_heads);
   p.tiles = ((c.prefix_count << c.page_shift) + kBN - 1) / kBN;
   const int64_t blocks = (c.sequences + 2 * p.per_tile - 1) / (2 * p.per_tile);
-  p.units = blocks * c.kv_heads * p.tiles;
+  p.items_count = blocks * c.kv_heads;
+  p.units = p.items_count * p.tiles;
   p.ctas = static_cast<int>(std::min<int64_t>(p.units, sm_count()));
   return p;
 }
@@ -1008,6 +1010,7 @@ cudaError_t launch_shared_keys(const PagedCache& c, const void* q, const void* k
   if (e != cudaSuccess) return e;
   a.records = plan.records;
   a.whole = plan.whole;
+  a.items = plan.items;
   a.shared_keys = c.prefix_count << c.page_shift;
   return launch<true>(plan.ctas, maps, a, stream);
 }
