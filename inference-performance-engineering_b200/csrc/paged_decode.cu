@@ -335,6 +335,8 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_merge_kernel(const Dec
   join_parts(parts, out);
 }
 
+std::atomic<uint64_t> shared_memory_allowed{0};  // of paged_decode_kernel, by device
+
 size_t items_bytes(int64_t items) { return (static_cast<size_t>(items) * sizeof(int2) + 255) / 256 * 256; }
 
 DecodeArgs decode_args(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out, int q_heads,
@@ -370,8 +372,7 @@ size_t paged_decode_workspace_bytes(int sequences, int q_heads, int kv_heads) {
 
 cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
                                 int q_heads, void* workspace, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kSmem));
+  cudaError_t e = allow_shared_memory(paged_decode_kernel, kSmem, &shared_memory_allowed);
   if (e != cudaSuccess) return e;
   const DecodeArgs a = decode_args(c, q, k_pages, v_pages, out, q_heads, workspace);
   const int grid = decode_grid(c);
@@ -391,8 +392,7 @@ size_t shared_prefix_workspace_bytes(const PagedCache& c, int q_heads) {
 cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
                                  int q_heads, void* workspace, cudaStream_t stream) {
   if (c.prefix_count == 0) return launch_paged_decode(c, q, k_pages, v_pages, out, q_heads, workspace, stream);
-  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kSmem));
+  cudaError_t e = allow_shared_memory(paged_decode_kernel, kSmem, &shared_memory_allowed);
   if (e != cudaSuccess) return e;
   const size_t rows = static_cast<size_t>(c.sequences) * q_heads * kRecord;
   SharedKeys shared = shared_keys_plan(c, q_heads);

@@ -958,8 +958,8 @@ cudaError_t prepare(const PagedCache& c, const void* q, const void* k_pages, con
 
 template <bool kShared>
 cudaError_t launch(int64_t grid, const Maps& maps, const PrefillArgs& a, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<kShared>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kSmem));
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_shared_memory(paged_prefill_kernel<kShared>, kSmem, &allowed);
   if (e != cudaSuccess) return e;
   paged_prefill_kernel<kShared><<<static_cast<unsigned>(grid), kThreads, kSmem, stream>>>(maps.q, maps.k, maps.v, a);
   return cudaGetLastError();

@@ -3,7 +3,10 @@
 #pragma once
 
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 
 namespace ipe {
 
@@ -18,5 +21,19 @@ bool make_map_3d(CUtensorMap* map, const void* ptr, int k, int rows, int slices,
                  int box_k, int box_slices = 1);
 
 int sm_count();
+
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device. `done` remembers the devices
+// on which that has been said (one word per kernel, zero at first).
+template <typename Kernel>
+cudaError_t allow_shared_memory(Kernel kernel, size_t bytes, std::atomic<uint64_t>* done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (done->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 }  // namespace ipe

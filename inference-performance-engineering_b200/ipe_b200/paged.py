@@ -25,25 +25,25 @@ Every function runs on the current stream of its tensors' device. Outputs must n
 
 from __future__ import annotations
 
-import contextlib
 import functools
 
 import torch
 
 from ipe_b200 import _native as nat
 
-_SAME_DEVICE = contextlib.nullcontext()
+# The checks run on every call of a step whose kernels take a few microseconds, so what follows from the
+# tensors' shapes alone (their agreement, the sizes the kernels get, the workspace) is worked out once per
+# set of shapes.
 
 
-def _device(name: str, pages: torch.Tensor) -> int:
-    if not isinstance(pages, torch.Tensor) or not pages.is_cuda:
-        raise ValueError(f"{name}: expected CUDA tensors")
-    return pages.get_device()
-
-
-def _check(name: str, device: int, dtype: torch.dtype, **tensors: torch.Tensor) -> None:
+def _check(name: str, dtype: torch.dtype, labels: tuple[str, ...], tensors: tuple[torch.Tensor, ...], device: int) -> None:
     """Every tensor is contiguous, on CUDA device `device` and of `dtype`."""
-    for label, t in tensors.items():
+    for t in tensors:
+        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.is_contiguous()):
+            break
+    else:
+        return
+    for label, t in zip(labels, tensors):
         if not isinstance(t, torch.Tensor) or t.get_device() != device:
             raise ValueError(f"{name}: {label} must be a CUDA tensor, on the device of the others")
         if t.dtype is not dtype:
@@ -52,42 +52,60 @@ def _check(name: str, device: int, dtype: torch.dtype, **tensors: torch.Tensor) 
             raise ValueError(f"{name}: {label} must be contiguous")
 
 
-def _cache(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
-           lengths: torch.Tensor) -> tuple[int, int, int, int, int]:
-    """(pages, KV heads, page size, sequences, pages per sequence)."""
-    if k_pages.dim() != 4 or k_pages.shape[3] != 128 or v_pages.shape != k_pages.shape:
+def _device(name: str, pages: torch.Tensor) -> int:
+    if not isinstance(pages, torch.Tensor) or not pages.is_cuda:
+        raise ValueError(f"{name}: expected CUDA tensors")
+    return pages.get_device()
+
+
+def _cache_sizes(name, k_pages, v_pages, page_table, lengths):
+    """(pages, KV heads, page size, sequences, pages per sequence) from the shapes."""
+    if len(k_pages) != 4 or k_pages[3] != 128 or v_pages != k_pages:
         raise ValueError(f"{name}: k_pages and v_pages must share a shape [pages, KV heads, page size, 128]")
-    if page_table.dim() != 2 or lengths.shape != page_table.shape[:1]:
+    if len(page_table) != 2 or lengths != page_table[:1]:
         raise ValueError(f"{name}: page_table must be [sequences, pages per sequence] and lengths [sequences]")
-    pages, kv_heads, page_size, _ = k_pages.shape
-    return pages, kv_heads, page_size, page_table.shape[0], page_table.shape[1]
+    return k_pages[0], k_pages[1], k_pages[2], page_table[0], page_table[1]
 
 
-def _heads(name: str, q: torch.Tensor, out: torch.Tensor, rows: int | None = None) -> int:
-    if q.dim() != 3 or q.shape[2] != 128 or (rows is not None and q.shape[0] != rows):
-        raise ValueError(f"{name}: q must be [{'rows' if rows is None else rows}, query heads, 128]")
-    if out.shape != (q.shape[0], q.shape[1] * 128):
+@functools.lru_cache(maxsize=4096)
+def _append_sizes(name, qkv, q_norm, k_norm, cos, sin, cu_tokens, lengths, page_table, q_out, k_pages, v_pages):
+    sizes = _cache_sizes(name, k_pages, v_pages, page_table, lengths)
+    if len(q_out) != 3 or q_out[2] != 128 or qkv != (q_out[0], (q_out[1] + 2 * sizes[1]) * 128):
+        raise ValueError(f"{name}: qkv must be [rows, (query heads + 2 * KV heads) * 128] and q_out [rows, query heads, 128]")
+    if q_norm != (128,) or k_norm != (128,) or len(cos) != 2 or cos[1] != 128 or sin != cos:
+        raise ValueError(f"{name}: q_norm and k_norm must be [128], cos and sin [positions, 128]")
+    if cu_tokens != (sizes[3] + 1,):
+        raise ValueError(f"{name}: cu_tokens must be [sequences + 1]")
+    return sizes
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_sizes(name, device, q, k_pages, v_pages, page_table, lengths, out, cu_tokens=None, prefix_pages=None):
+    """The cache's sizes, the query heads and the workspace's bytes on CUDA device `device`."""
+    sizes = pages, kv_heads, page_size, sequences, width = _cache_sizes(name, k_pages, v_pages, page_table, lengths)
+    rows = sequences if cu_tokens is None else "rows"
+    if len(q) != 3 or q[2] != 128 or (cu_tokens is None and q[0] != sequences):
+        raise ValueError(f"{name}: q must be [{rows}, query heads, 128]")
+    if out != (q[0], q[1] * 128):
         raise ValueError(f"{name}: out must be [rows, query heads * 128]")
-    return q.shape[1]
+    if cu_tokens is not None and cu_tokens != (sequences + 1,):
+        raise ValueError(f"{name}: cu_tokens must be [sequences + 1]")
+    if prefix_pages is not None and (len(prefix_pages) != 1 or prefix_pages[0] > width):
+        raise ValueError(f"{name}: prefix_pages must be [prefix pages], no more than the {width} pages per sequence")
+    lib = nat.load()
+    if cu_tokens is not None:
+        workspace = lib.ipe_paged_prefill_attention_workspace(q[0], sequences, q[1], kv_heads)
+    elif prefix_pages is not None:
+        workspace = lib.ipe_shared_prefix_attention_workspace(sequences, q[1], kv_heads, page_size, prefix_pages[0])
+    else:
+        workspace = lib.ipe_paged_decode_attention_workspace(sequences, q[1], kv_heads)
+    return (*sizes, q[1], int(workspace))
 
 
-def _on(device: int):
-    """The guard under which a call's stream, workspace and launches belong to `device`."""
-    return _SAME_DEVICE if device == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(entry: str, device: int, *sizes: int) -> int:
-    return int(getattr(nat.load(), entry)(*sizes))
-
-
-def _workspace(device: int, entry: str, *sizes: int) -> torch.Tensor:
-    """The call's own scratch, from torch's allocator: calls on other streams, and captured ones, have others."""
-    return torch.empty(_workspace_bytes(entry, device, *sizes), dtype=torch.uint8, device=device)
+def _elsewhere(device, function, *args):
+    """The call under its tensors' device, to which its launches, workspace and stream belong."""
+    with torch.cuda.device(device):
+        return function(*args)
 
 
 def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor, cos: torch.Tensor,
@@ -102,22 +120,24 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: t
     """
     name = "paged_qk_norm_rope_append"
     device = _device(name, k_pages)
+    if device != torch._C._cuda_getDevice():
+        return _elsewhere(device, paged_qk_norm_rope_append, qkv, q_norm, k_norm, cos, sin, cu_tokens, lengths, page_table, eps,
+                          q_out, k_pages, v_pages)
     table = torch.float32 if getattr(cos, "dtype", None) is torch.float32 else torch.bfloat16
-    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, qkv=qkv, q_norm=q_norm, k_norm=k_norm, q_out=q_out)
-    _check(name, device, table, cos=cos, sin=sin)
-    _check(name, device, torch.int32, cu_tokens=cu_tokens, lengths=lengths, page_table=page_table)
-    pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
-    if q_out.dim() != 3 or q_out.shape[2] != 128 or qkv.shape != (q_out.shape[0], (q_out.shape[1] + 2 * kv_heads) * 128):
-        raise ValueError(f"{name}: qkv must be [rows, (query heads + 2 * KV heads) * 128] and q_out [rows, query heads, 128]")
-    if q_norm.shape != (128,) or k_norm.shape != (128,) or cos.dim() != 2 or cos.shape[1] != 128 or sin.shape != cos.shape:
-        raise ValueError(f"{name}: q_norm and k_norm must be [128], cos and sin [positions, 128]")
-    if cu_tokens.shape != (sequences + 1,):
-        raise ValueError(f"{name}: cu_tokens must be [sequences + 1]")
-    with _on(device):
-        nat.call("ipe_paged_qk_norm_rope_append", qkv.data_ptr(), q_out.shape[0], q_out.shape[1], kv_heads,
-                 q_norm.data_ptr(), k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), int(table is torch.float32),
-                 cos.shape[0], cu_tokens.data_ptr(), lengths.data_ptr(), page_table.data_ptr(), sequences, width,
-                 q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size, float(eps), _stream(device))
+    _check(name, torch.bfloat16, ("k_pages", "v_pages", "qkv", "q_norm", "k_norm", "q_out"),
+           (k_pages, v_pages, qkv, q_norm, k_norm, q_out), device)
+    _check(name, table, ("cos", "sin"), (cos, sin), device)
+    _check(name, torch.int32, ("cu_tokens", "lengths", "page_table"), (cu_tokens, lengths, page_table), device)
+    rows = q_out.shape
+    pages, kv_heads, page_size, sequences, width = _append_sizes(
+        name, qkv.shape, q_norm.shape, k_norm.shape, cos.shape, sin.shape, cu_tokens.shape, lengths.shape,
+        page_table.shape, rows, k_pages.shape, v_pages.shape)
+    status = nat.load().ipe_paged_qk_norm_rope_append(qkv.data_ptr(), rows[0], rows[1], kv_heads, q_norm.data_ptr(),
+             k_norm.data_ptr(), cos.data_ptr(), sin.data_ptr(), 1 if table is torch.float32 else 0, cos.shape[0],
+             cu_tokens.data_ptr(), lengths.data_ptr(), page_table.data_ptr(), sequences, width, q_out.data_ptr(),
+             k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size, eps, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        nat.check(status, "ipe_paged_qk_norm_rope_append")
     return q_out
 
 
@@ -127,15 +147,18 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     token q [S, Hq, 128] each, 1 to 8 query heads per KV head. A sequence of length 0 gives zeros."""
     name = "paged_decode_attention"
     device = _device(name, k_pages)
-    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
-    _check(name, device, torch.int32, page_table=page_table, lengths=lengths)
-    pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
-    q_heads = _heads(name, q, out, sequences)
-    with _on(device):
-        ws = _workspace(device, "ipe_paged_decode_attention_workspace", sequences, q_heads, kv_heads)
-        nat.call("ipe_paged_decode_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                 page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), sequences, q_heads, kv_heads, pages,
-                 page_size, width, ws.data_ptr(), ws.numel(), _stream(device))
+    if device != torch._C._cuda_getDevice():
+        return _elsewhere(device, paged_decode_attention, q, k_pages, v_pages, page_table, lengths, out)
+    _check(name, torch.bfloat16, ("k_pages", "v_pages", "q", "out"), (k_pages, v_pages, q, out), device)
+    _check(name, torch.int32, ("page_table", "lengths"), (page_table, lengths), device)
+    pages, kv_heads, page_size, sequences, width, q_heads, need = _attention_sizes(
+        name, device, q.shape, k_pages.shape, v_pages.shape, page_table.shape, lengths.shape, out.shape)
+    workspace = k_pages.new_empty(need, dtype=torch.uint8)  # the call's own: other streams and graphs have others
+    status = nat.load().ipe_paged_decode_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+             lengths.data_ptr(), out.data_ptr(), sequences, q_heads, kv_heads, pages, page_size, width,
+             workspace.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        nat.check(status, "ipe_paged_decode_attention")
     return out
 
 
@@ -145,17 +168,19 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     sequence s brings sees keys 0 .. lengths[s] - n + i. out [rows, Hq * 128]; 1 to 8 query heads per KV head."""
     name = "paged_prefill_attention"
     device = _device(name, k_pages)
-    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
-    _check(name, device, torch.int32, page_table=page_table, cu_tokens=cu_tokens, lengths=lengths)
-    pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
-    q_heads = _heads(name, q, out)
-    if cu_tokens.shape != (sequences + 1,):
-        raise ValueError(f"{name}: cu_tokens must be [sequences + 1]")
-    with _on(device):
-        ws = _workspace(device, "ipe_paged_prefill_attention_workspace", q.shape[0], sequences, q_heads, kv_heads)
-        nat.call("ipe_paged_prefill_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                 page_table.data_ptr(), cu_tokens.data_ptr(), lengths.data_ptr(), out.data_ptr(), q.shape[0], sequences,
-                 q_heads, kv_heads, pages, page_size, width, ws.data_ptr(), ws.numel(), _stream(device))
+    if device != torch._C._cuda_getDevice():
+        return _elsewhere(device, paged_prefill_attention, q, k_pages, v_pages, page_table, cu_tokens, lengths, out)
+    _check(name, torch.bfloat16, ("k_pages", "v_pages", "q", "out"), (k_pages, v_pages, q, out), device)
+    _check(name, torch.int32, ("page_table", "cu_tokens", "lengths"), (page_table, cu_tokens, lengths), device)
+    rows = q.shape
+    pages, kv_heads, page_size, sequences, width, q_heads, need = _attention_sizes(
+        name, device, rows, k_pages.shape, v_pages.shape, page_table.shape, lengths.shape, out.shape, cu_tokens.shape)
+    workspace = k_pages.new_empty(need, dtype=torch.uint8)
+    status = nat.load().ipe_paged_prefill_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+             cu_tokens.data_ptr(), lengths.data_ptr(), out.data_ptr(), rows[0], sequences, q_heads, kv_heads, pages,
+             page_size, width, workspace.data_ptr(), need, torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        nat.check(status, "ipe_paged_prefill_attention")
     return out
 
 
@@ -167,17 +192,18 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     lengths [S] count the prefix; a sequence that ends inside the prefix sees its own lengths[s] keys of it."""
     name = "shared_prefix_attention"
     device = _device(name, k_pages)
-    _check(name, device, torch.bfloat16, k_pages=k_pages, v_pages=v_pages, q=q, out=out)
-    _check(name, device, torch.int32, prefix_pages=prefix_pages, page_table=page_table, lengths=lengths)
-    pages, kv_heads, page_size, sequences, width = _cache(name, k_pages, v_pages, page_table, lengths)
-    q_heads = _heads(name, q, out, sequences)
-    if prefix_pages.dim() != 1 or prefix_pages.shape[0] > width:
-        raise ValueError(f"{name}: prefix_pages must be [prefix pages], no more than the {width} pages per sequence")
-    with _on(device):
-        ws = _workspace(device, "ipe_shared_prefix_attention_workspace", sequences, q_heads, kv_heads, page_size,
-                        prefix_pages.shape[0])
-        nat.call("ipe_shared_prefix_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                 prefix_pages.data_ptr(), prefix_pages.shape[0], page_table.data_ptr(), lengths.data_ptr(),
-                 out.data_ptr(), sequences, q_heads, kv_heads, pages, page_size, width, ws.data_ptr(), ws.numel(),
-                 _stream(device))
+    if device != torch._C._cuda_getDevice():
+        return _elsewhere(device, shared_prefix_attention, q, k_pages, v_pages, prefix_pages, page_table, lengths, out)
+    _check(name, torch.bfloat16, ("k_pages", "v_pages", "q", "out"), (k_pages, v_pages, q, out), device)
+    _check(name, torch.int32, ("prefix_pages", "page_table", "lengths"), (prefix_pages, page_table, lengths), device)
+    prefix = prefix_pages.shape
+    pages, kv_heads, page_size, sequences, width, q_heads, need = _attention_sizes(
+        name, device, q.shape, k_pages.shape, v_pages.shape, page_table.shape, lengths.shape, out.shape, None, prefix)
+    workspace = k_pages.new_empty(need, dtype=torch.uint8)
+    status = nat.load().ipe_shared_prefix_attention(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+             prefix_pages.data_ptr(), prefix[0], page_table.data_ptr(), lengths.data_ptr(), out.data_ptr(), sequences,
+             q_heads, kv_heads, pages, page_size, width, workspace.data_ptr(), need,
+             torch._C._cuda_getCurrentRawStream(device))
+    if status:
+        nat.check(status, "ipe_shared_prefix_attention")
     return out
