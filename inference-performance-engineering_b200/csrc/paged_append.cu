@@ -8,8 +8,10 @@
 // Bound by memory: 256 bytes in and out per head slot. A warp has a few consecutive tokens, or a share of one
 // token's slots where there are few: enough warps to fill the GPU once, so the chain of lookups that a place
 // takes (sequence, length, page; a lane per token) is paid once per warp and behind the first rows' loads.
-// 16 lanes per row, each with elements 4j..4j+3 and 64+4j..64+4j+3, so the rotation stays in the lane; a token's
-// cosines and sines stay in registers over its rows.
+// Its rows are one contiguous run of qkv, which bulk copies bring into a ring of 4 KB pieces, so loads cost no
+// instructions and never wait for arithmetic. 16 lanes per row, each with elements 4j..4j+3 and
+// 64+4j..64+4j+3, so the rotation stays in the lane: o_lo = r (x_lo a_lo - x_hi b_lo), o_hi = r (x_hi a_hi +
+// x_lo b_hi) with a = w cos, b = w sin formed once per token and kind of head.
 #include <algorithm>
 
 #include "launch.h"
@@ -21,23 +23,28 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kAhead = 2;       // pairs of rows in flight
-constexpr int kMostSplit = 8;   // warps that share a token's slots
+constexpr int kPiece = 16;       // rows of a bulk copy
+constexpr int kStages = 2;       // pieces of a warp in flight
+constexpr int kBlocksPerSm = 3;  // by shared memory and registers
+constexpr int kMostSplit = 8;    // warps that share a token's slots
 constexpr int kMostTokens = 32;  // of a warp
+constexpr size_t kSmem = static_cast<size_t>(kWarps) * kStages * kPiece * 256;
 
-__device__ __forceinline__ void unpack4(const uint2& v, float* f) {
-  f[0] = __uint_as_float(v.x << 16);
-  f[1] = __uint_as_float(v.x & 0xffff0000u);
-  f[2] = __uint_as_float(v.y << 16);
-  f[3] = __uint_as_float(v.y & 0xffff0000u);
+// Four elements as two pairs.
+__device__ __forceinline__ void unpack4(const uint2& v, uint64_t* f) {
+  f[0] = pair(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u));
+  f[1] = pair(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
 }
-__device__ __forceinline__ void load4(const bf16* p, float* f) { unpack4(__ldg(reinterpret_cast<const uint2*>(p)), f); }
-__device__ __forceinline__ void load4(const float* p, float* f) {
+__device__ __forceinline__ void load4(const bf16* p, uint64_t* f) { unpack4(__ldg(reinterpret_cast<const uint2*>(p)), f); }
+__device__ __forceinline__ void load4(const float* p, uint64_t* f) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-  f[0] = a.x;
-  f[1] = a.y;
-  f[2] = a.z;
-  f[3] = a.w;
+  f[0] = pair(a.x, a.y);
+  f[1] = pair(a.z, a.w);
+}
+__device__ __forceinline__ uint32_t pack2(uint64_t v) {
+  float lo, hi;
+  unpair(v, &lo, &hi);
+  return pack_bf16x2(lo, hi);
 }
 
 // The sequence that brings token `t`, or -1: each lane for its own token.
@@ -74,98 +81,120 @@ __device__ __forceinline__ Place place_of(const PagedCache& c, int s, int t, int
   return p;
 }
 
-struct Row {
-  uint2 lo, hi;  // a lane's elements of a row: 4j.., 64 + 4j..
-};
-
 template <typename Table>
-__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const PagedCache c, const bf16* __restrict__ qkv,
-                                                                   int tokens, int per_warp, int split, int q_heads,
-                                                                   const bf16* __restrict__ q_norm,
-                                                                   const bf16* __restrict__ k_norm,
-                                                                   const Table* __restrict__ cos_t,
-                                                                   const Table* __restrict__ sin_t, int64_t table_rows,
-                                                                   bf16* __restrict__ q_out, bf16* __restrict__ k_pages,
-                                                                   bf16* __restrict__ v_pages, float eps) {
-  const int warp = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+    paged_append_kernel(const PagedCache c, const bf16* __restrict__ qkv, int tokens, int per_warp, int split, int q_heads,
+                        const bf16* __restrict__ q_norm, const bf16* __restrict__ k_norm, const Table* __restrict__ cos_t,
+                        const Table* __restrict__ sin_t, int64_t table_rows, bf16* __restrict__ q_out,
+                        bf16* __restrict__ k_pages, bf16* __restrict__ v_pages, float eps) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint64_t bars[kWarps][kStages];
+  const int local = threadIdx.x >> 5, lane = threadIdx.x & 31, warp = blockIdx.x * kWarps + local;
   const int t0 = warp / split * per_warp, mine = min(per_warp, tokens - t0);
-  if (mine <= 0) return;
   const int slots = q_heads + 2 * c.kv_heads, share = (slots + split - 1) / split;
-  const int slot0 = warp % split * share, slot1 = min(slots, slot0 + share);
-  const int team = lane >> 4, d0 = (lane & 15) * 4;
-  const bf16* src = qkv + static_cast<int64_t>(t0) * slots * 128 + d0;
-  Row raw[kAhead];
-  auto load = [&](int token, int slot) {  // this lane's part of row `slot + team`
-    Row x{make_uint2(0, 0), make_uint2(0, 0)};
-    if (token < mine && slot + team < slot1) {
-      const bf16* p = src + (token * slots + slot + team) * 128;
-      x.lo = __ldcs(reinterpret_cast<const uint2*>(p));
-      x.hi = __ldcs(reinterpret_cast<const uint2*>(p + 64));
-    }
-    return x;
+  const int slot0 = warp % split * share, width = min(slots, slot0 + share) - slot0;  // of the slots
+  const int rows = mine > 0 && width > 0 ? mine * width : 0;  // one run: several tokens only with all their slots
+  if (rows == 0) return;
+  unsigned char* ring = smem + local * (kStages * kPiece * 256);
+  const bf16* src = qkv + (static_cast<int64_t>(t0) * slots + slot0) * 128;
+  auto fetch = [&](int piece) {
+    const int n = min(kPiece, rows - piece * kPiece) * 256;
+    uint64_t* bar = &bars[local][piece % kStages];
+    mbar_expect_tx(bar, n);
+    bulk_copy(smem_addr(ring) + piece % kStages * (kPiece * 256), src + static_cast<int64_t>(piece) * (kPiece * 128), n, bar);
   };
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) raw[u] = load(0, slot0 + 2 * u);
+  const int pieces = (rows + kPiece - 1) / kPiece;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(&bars[local][i], 1);
+    fence_barrier_init();
+    for (int i = 0; i < min(kStages, pieces); ++i) fetch(i);
+  }
   Place own{-1, 0, 0};
   if (per_warp == 1)
     own = place_of(c, find_sequence(c.cu_tokens, c.sequences, t0), t0, table_rows);
   else if (lane < mine)
     own = place_of(c, sequence_of(c, t0 + lane), t0 + lane, table_rows);
-  const uint2 wq_lo = __ldg(reinterpret_cast<const uint2*>(q_norm + d0)), wq_hi = __ldg(reinterpret_cast<const uint2*>(q_norm + 64 + d0));
-  const uint2 wk_lo = __ldg(reinterpret_cast<const uint2*>(k_norm + d0)), wk_hi = __ldg(reinterpret_cast<const uint2*>(k_norm + 64 + d0));
+  __syncwarp();
 
-  for (int token = 0; token < mine; ++token) {
-    const int position = __shfl_sync(0xffffffffu, own.position, token);
-    const bool stored = __shfl_sync(0xffffffffu, own.stored, token);
-    const int64_t row0 = __shfl_sync(0xffffffffu, own.row, token);
-    float cos_lo[4], cos_hi[4], sin_lo[4], sin_hi[4];
-    const int64_t at = static_cast<int64_t>(max(position, 0)) * 128 + d0;
-    load4(cos_t + at, cos_lo);
-    load4(cos_t + at + 64, cos_hi);
-    load4(sin_t + at, sin_lo);
-    load4(sin_t + at + 64, sin_hi);
-    for (int base = slot0; base < slot1; base += 2 * kAhead) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const Row row = raw[u];
-        // the row that takes this place next: of this token, or of the next
-        raw[u] = base + 2 * kAhead < slot1 ? load(token, base + 2 * (kAhead + u)) : load(token + 1, slot0 + 2 * u);
-        const int first = base + 2 * u, slot = first + team;  // slots first, first + 1
-        if (first >= slot1) continue;
-        const bool is_q = slot < q_heads, is_v = slot >= q_heads + c.kv_heads;
-        Row out = row;
-        if (first < q_heads + c.kv_heads) {  // not two value heads
-          float lo[4], hi[4], wl[4], wh[4];
-          unpack4(row.lo, lo);
-          unpack4(row.hi, hi);
-          unpack4(is_q ? wq_lo : wk_lo, wl);
-          unpack4(is_q ? wq_hi : wk_hi, wh);
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) ss += lo[i] * lo[i] + hi[i] * hi[i];
-#pragma unroll
-          for (int k = 8; k > 0; k >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, k);
-          const float r = rsqrtf(ss * (1.f / 128.f) + eps);
-          float a[4], b[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float l = lo[i] * r * wl[i], h = hi[i] * r * wh[i];
-            a[i] = l * cos_lo[i] - h * sin_lo[i];
-            b[i] = h * cos_hi[i] + l * sin_hi[i];
-          }
-          if (!is_v) {
-            out.lo = make_uint2(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]));
-            out.hi = make_uint2(pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]));
-          }
-        }
-        if (position < 0 || slot >= slot1 || (!is_q && !stored)) continue;
-        const int h = slot - q_heads - (is_v ? c.kv_heads : 0);
-        bf16* dst = is_q ? q_out + (static_cast<int64_t>(t0 + token) * q_heads + slot) * 128
-                         : (is_v ? v_pages : k_pages) + (row0 + (static_cast<int64_t>(h) << c.page_shift)) * 128;
-        *reinterpret_cast<uint2*>(dst + d0) = out.lo;
-        *reinterpret_cast<uint2*>(dst + 64 + d0) = out.hi;
-      }
+  const int team = lane >> 4, d0 = (lane & 15) * 4;
+  // This half warp's row, its slot counted from slot0, and what it shares with the rows after it until `left`, the
+  // slots of its token and kind of head from it on, runs out.
+  int token = 0, slot = team, left = 0;
+  bool normed = false, writes = false;
+  uint64_t a_lo[2], a_hi[2], b_lo[2], b_hi[2];
+  bf16* dst = nullptr;  // this lane's part of the row
+  int64_t stride = 0;   // elements from a head's row to the next
+  for (int piece = 0; piece < pieces; ++piece) {
+    if (!mbar_wait(&bars[local][piece % kStages], (piece / kStages) & 1, c.err)) {
+      for (int i = piece + 1; i < min(piece + kStages, pieces); ++i) mbar_wait(&bars[local][i % kStages], (i / kStages) & 1, c.err);
+      return;  // the copies in flight have had their time too
     }
+    const unsigned char* in = ring + piece % kStages * (kPiece * 256) + team * 256 + d0 * 2;
+    const int n = min(kPiece, rows - piece * kPiece);
+#pragma unroll 4
+    for (int k = 0; k < kPiece / 2; ++k) {
+      if (2 * k >= n) break;
+      uint2 lo = *reinterpret_cast<const uint2*>(in + k * 512), hi = *reinterpret_cast<const uint2*>(in + k * 512 + 128);
+      if (__any_sync(0xffffffffu, left <= 0)) {  // another token, or another kind of head
+        while (slot >= width) {
+          slot -= width;
+          ++token;
+        }
+        const int head = slot0 + slot, kind = (head >= q_heads) + (head >= q_heads + c.kv_heads);
+        const int from = min(token, 31), first = kind == 0 ? 0 : q_heads + (kind - 1) * c.kv_heads;
+        const int position = __shfl_sync(0xffffffffu, own.position, from);
+        const bool stored = __shfl_sync(0xffffffffu, own.stored, from);
+        const int64_t row0 = __shfl_sync(0xffffffffu, own.row, from);
+        left = min(width - slot, first + (kind == 0 ? q_heads : c.kv_heads) - head);
+        normed = kind < 2;
+        writes = position >= 0 && (kind == 0 || stored);
+        stride = kind == 0 ? 128 : static_cast<int64_t>(128) << c.page_shift;
+        dst = (kind == 0 ? q_out + static_cast<int64_t>(t0 + token) * q_heads * 128 : (kind == 1 ? k_pages : v_pages) + row0 * 128) +
+              (head - first) * stride + d0;
+        const int64_t angle = static_cast<int64_t>(max(position, 0)) * 128 + d0;
+        const bf16* w = kind == 0 ? q_norm : k_norm;
+        uint64_t w_lo[2], w_hi[2];
+        load4(w + d0, w_lo);
+        load4(w + 64 + d0, w_hi);
+        load4(cos_t + angle, a_lo);
+        load4(cos_t + angle + 64, a_hi);
+        load4(sin_t + angle, b_lo);
+        load4(sin_t + angle + 64, b_hi);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          a_lo[i] = mul2(a_lo[i], w_lo[i]);
+          a_hi[i] = mul2(a_hi[i], w_hi[i]);
+          b_lo[i] = mul2(mul2(b_lo[i], w_hi[i]), pair(-1.f, -1.f));
+          b_hi[i] = mul2(b_hi[i], w_lo[i]);
+        }
+      }
+      if (__any_sync(0xffffffffu, normed)) {
+        uint64_t x[2], y[2];
+        unpack4(lo, x);
+        unpack4(hi, y);
+        const uint64_t ss2 = fma2(y[1], y[1], fma2(y[0], y[0], fma2(x[1], x[1], mul2(x[0], x[0]))));
+        float ss, more, r;
+        unpair(ss2, &ss, &more);
+        ss += more;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ss * (1.f / 128.f) + eps));
+        if (normed) {
+          const uint64_t r2 = pair(r, r);
+          lo = make_uint2(pack2(mul2(r2, fma2(y[0], b_lo[0], mul2(x[0], a_lo[0])))), pack2(mul2(r2, fma2(y[1], b_lo[1], mul2(x[1], a_lo[1])))));
+          hi = make_uint2(pack2(mul2(r2, fma2(x[0], b_hi[0], mul2(y[0], a_hi[0])))), pack2(mul2(r2, fma2(x[1], b_hi[1], mul2(y[1], a_hi[1])))));
+        }
+      }
+      if (writes && 2 * k + team < n) {
+        *reinterpret_cast<uint2*>(dst) = lo;
+        *reinterpret_cast<uint2*>(dst + 64) = hi;
+      }
+      slot += 2;
+      left -= 2;
+      dst += 2 * stride;
+    }
+    __syncwarp();
+    if (lane == 0 && piece + kStages < pieces) fetch(piece + kStages);
   }
 }
 
@@ -177,19 +206,23 @@ cudaError_t launch_paged_append(const PagedCache& c, const void* qkv, int64_t to
                                 cudaStream_t stream) {
   const auto x = static_cast<const bf16*>(qkv), qn = static_cast<const bf16*>(q_norm), kn = static_cast<const bf16*>(k_norm);
   const auto q = static_cast<bf16*>(q_out), k = static_cast<bf16*>(k_pages), v = static_cast<bf16*>(v_pages);
-  // warps that fill the GPU once (32 per SM): shares of a token where there are few tokens, several tokens where many
-  const int64_t fill = 32 * static_cast<int64_t>(sm_count());
+  // warps that fill the GPU once: shares of a token where there are few tokens, several tokens where many
+  const int64_t fill = static_cast<int64_t>(kBlocksPerSm) * kWarps * sm_count();
   int split = 1;
   while (split < kMostSplit && 2 * split * tokens <= fill) split *= 2;
   const int per_warp = static_cast<int>(std::min<int64_t>(kMostTokens, (tokens + fill - 1) / fill));
   const int64_t warps = (tokens + per_warp - 1) / per_warp * split;
   const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
   const int n = static_cast<int>(tokens);
+  static std::atomic<uint64_t> allowed[2] = {{0}, {0}};
+  cudaError_t e = fp32_tables ? allow_shared_memory(paged_append_kernel<float>, kSmem, &allowed[1])
+                              : allow_shared_memory(paged_append_kernel<bf16>, kSmem, &allowed[0]);
+  if (e != cudaSuccess) return e;
   if (fp32_tables)
-    paged_append_kernel<float><<<grid, kThreads, 0, stream>>>(c, x, n, per_warp, split, q_heads, qn, kn, static_cast<const float*>(cos_t),
+    paged_append_kernel<float><<<grid, kThreads, kSmem, stream>>>(c, x, n, per_warp, split, q_heads, qn, kn, static_cast<const float*>(cos_t),
                                                               static_cast<const float*>(sin_t), table_rows, q, k, v, eps);
   else
-    paged_append_kernel<bf16><<<grid, kThreads, 0, stream>>>(c, x, n, per_warp, split, q_heads, qn, kn, static_cast<const bf16*>(cos_t),
+    paged_append_kernel<bf16><<<grid, kThreads, kSmem, stream>>>(c, x, n, per_warp, split, q_heads, qn, kn, static_cast<const bf16*>(cos_t),
                                                              static_cast<const bf16*>(sin_t), table_rows, q, k, v, eps);
   return cudaGetLastError();
 }

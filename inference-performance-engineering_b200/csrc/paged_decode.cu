@@ -10,7 +10,10 @@
 // piece. S = K q^T and O^T = V^T P^T as m16n8k16 products with the keys (then the head's dimensions) as
 // the 16 rows and the query heads as the 8 columns, so a thread's scores and its output accumulators
 // belong to the same two heads. P enters as two bf16 terms (value and remainder), so the weights keep
-// 16 bits: the products are idle anyway. K and V come through per-warp rings of cp.async copies, which
+// 16 bits: the products are idle anyway. What a warp waits for (its loads, the chain from scores to weights)
+// the other warps of the SM fill: 3 CTAs with 2 units in flight each against 2 with 3 measured 101.5 and
+// 110.8 us for 160 rows behind a shared prefix, 111.0 and 114.8 for 64 rows of 700 to 12289 keys (6.1 TB/s).
+// K and V come through per-warp rings of cp.async copies, which
 // fill keys past the sequence's end with zeros without reading them: what an unused row holds (NaN,
 // say) never meets a weight of zero.
 #include <algorithm>
@@ -25,14 +28,15 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnit = 16 * kWarps;       // keys
-constexpr int kStages = 3;               // units in flight per CTA
+constexpr int kStages = 2;               // units in flight per CTA
 constexpr int kStageBytes = 2 * 16 * 256;  // one warp's keys and values of a unit
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 3;  // by registers
 constexpr int kHeads = 8;                // columns of the products
 constexpr int kNothing = -2;             // an item without keys
 constexpr int kMergeStride = 132;        // floats; spreads a warp's 4 head pairs over the banks
-constexpr size_t kSmem = static_cast<size_t>(kStages) * kWarps * kStageBytes +
-                         static_cast<size_t>(kWarps) * kHeads * kMergeStride * sizeof(float);
+constexpr size_t smem_bytes(int group) {
+  return static_cast<size_t>(kStages) * kWarps * kStageBytes + static_cast<size_t>(kWarps) * group * kMergeStride * sizeof(float);
+}
 
 struct DecodeArgs {
   PagedCache c;
@@ -141,15 +145,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       const int64_t row0 = c.page_row(page, ahead.h) + (key0 & (c.page_size() - 1));
       const int chunk = lane & 15;
       const uint32_t dst = ring + stage * (kWarps * kStageBytes);
-      const bf16* ks = a.k + row0 * 128 + chunk * 8;
-      const bf16* vs = a.v + row0 * 128 + chunk * 8;
+      // The 16 rows lie in one page, so every address is inside the cache; rows past the end are not read.
+      const bf16* ks = a.k + (row0 + (lane >> 4)) * 128 + chunk * 8;
+      const bf16* vs = a.v + (row0 + (lane >> 4)) * 128 + chunk * 8;
+      const uint32_t at = (lane >> 4) * 256 + ((chunk ^ (lane >> 4)) << 4);  // row r's chunk c: r * 256 + (c ^ r % 8) * 16
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int row = (lane >> 4) + 2 * i;
-        const uint32_t at = row * 256 + ((chunk ^ (row & 7)) << 4);
-        const bool real = row < valid;
-        cp_async16(dst + at, real ? ks + row * 128 : a.k, real ? 16 : 0);
-        cp_async16(dst + 4096 + at, real ? vs + row * 128 : a.v, real ? 16 : 0);
+        const uint32_t to = dst + i * 512 + (at ^ ((2 * i & 7) << 4));
+        const uint32_t bytes = (lane >> 4) + 2 * i < valid ? 16 : 0;
+        cp_async16(to, ks + i * 256, bytes);
+        cp_async16(to + 4096, vs + i * 256, bytes);
       }
       if (++issued < count) {
         ahead.advance(a);
@@ -221,12 +226,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
     const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1])), b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
     const uint32_t r0 = transpose8x8(pack_bf16x2(p[0] - bf16_round(p[0]), p[1] - bf16_round(p[1])));
     const uint32_t r1 = transpose8x8(pack_bf16x2(p[2] - bf16_round(p[2]), p[3] - bf16_round(p[3])));
+    if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] *= keep[i & 1];
+    }
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       uint32_t f0, f1, f2, f3;
       ldmatrix_x4_trans(f0, f1, f2, f3, vs + trow * 256 + (((2 * t + tcol) ^ (trow & 7)) << 4));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] *= keep[i & 1];
       mma16816(acc[t], f0, f1, f2, f3, b0, b1);
       mma16816(acc[t], f0, f1, f2, f3, r0, r1);
     }
@@ -243,11 +252,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
           stats[warp][g][0] = m[e];
           stats[warp][g][1] = l[e];
         }
-        float* o = merge + (warp * kHeads + g) * kMergeStride + (lane >> 2);
+        float* o = merge + (warp * group + g) * kMergeStride + (lane >> 2);
+        if (g < group) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          o[16 * t] = acc[t][e];
-          o[16 * t + 8] = acc[t][2 + e];
+          for (int t = 0; t < 8; ++t) {
+            o[16 * t] = acc[t][e];
+            o[16 * t + 8] = acc[t][2 + e];
+          }
         }
       }
       __syncthreads();
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         for (int w = 0; w < kWarps; ++w) {
           const float e = exp2_approx(stats[w][g][0] * kScaleLog2 - base);
           sum += e * stats[w][g][1];
-          o += e * merge[(w * kHeads + g) * kMergeStride + threadIdx.x];
+          o += e * merge[(w * group + g) * kMergeStride + threadIdx.x];
         }
         const int64_t row = static_cast<int64_t>(at.s) * a.q_heads + at.h * group + g;
         if (whole && !a.whole) {
@@ -337,6 +348,9 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_merge_kernel(const Dec
 
 std::atomic<uint64_t> shared_memory_allowed{0};  // of paged_decode_kernel, by device
 
+// CTAs per SM: the third fits beside the others' shared memory up to 5 query heads per KV head
+int ctas_per_sm(int group) { return group <= 5 ? kCtasPerSm : 2; }
+
 size_t items_bytes(int64_t items) { return (static_cast<size_t>(items) * sizeof(int2) + 255) / 256 * 256; }
 
 DecodeArgs decode_args(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out, int q_heads,
@@ -354,10 +368,10 @@ DecodeArgs decode_args(const PagedCache& c, const void* q, const void* k_pages, 
   return a;
 }
 
-int decode_grid(const PagedCache& c) {
+int decode_grid(const PagedCache& c, int q_heads) {
   const int64_t capacity = static_cast<int64_t>(c.max_pages - c.prefix_count) << c.page_shift;
   const int64_t most = static_cast<int64_t>(c.sequences) * c.kv_heads * ((capacity + kUnit - 1) / kUnit);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kCtasPerSm * sm_count(), most)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas_per_sm(q_heads / c.kv_heads) * sm_count(), most)));
 }
 
 dim3 merge_grid(const PagedCache& c, int q_heads) {
@@ -367,16 +381,16 @@ dim3 merge_grid(const PagedCache& c, int q_heads) {
 }  // namespace
 
 size_t paged_decode_workspace_bytes(int sequences, int q_heads, int kv_heads) {
-  return items_bytes(static_cast<int64_t>(sequences) * kv_heads) + static_cast<size_t>(kCtasPerSm * sm_count()) * 2 * (q_heads / kv_heads) * kRecord * sizeof(float);
+  return items_bytes(static_cast<int64_t>(sequences) * kv_heads) + static_cast<size_t>(ctas_per_sm(q_heads / kv_heads) * sm_count()) * 2 * (q_heads / kv_heads) * kRecord * sizeof(float);
 }
 
 cudaError_t launch_paged_decode(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
                                 int q_heads, void* workspace, cudaStream_t stream) {
-  cudaError_t e = allow_shared_memory(paged_decode_kernel, kSmem, &shared_memory_allowed);
+  cudaError_t e = allow_shared_memory(paged_decode_kernel, smem_bytes(kHeads), &shared_memory_allowed);
   if (e != cudaSuccess) return e;
   const DecodeArgs a = decode_args(c, q, k_pages, v_pages, out, q_heads, workspace);
-  const int grid = decode_grid(c);
-  paged_decode_kernel<<<grid, kThreads, kSmem, stream>>>(a);
+  const int grid = decode_grid(c, q_heads);
+  paged_decode_kernel<<<grid, kThreads, smem_bytes(q_heads / c.kv_heads), stream>>>(a);
   e = cudaGetLastError();
   if (e != cudaSuccess || (c.max_pages << c.page_shift) <= kUnit) return e;  // one unit per item: nothing to merge
   return launch_pdl(paged_decode_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a);
@@ -392,7 +406,7 @@ size_t shared_prefix_workspace_bytes(const PagedCache& c, int q_heads) {
 cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void* k_pages, const void* v_pages, void* out,
                                  int q_heads, void* workspace, cudaStream_t stream) {
   if (c.prefix_count == 0) return launch_paged_decode(c, q, k_pages, v_pages, out, q_heads, workspace, stream);
-  cudaError_t e = allow_shared_memory(paged_decode_kernel, kSmem, &shared_memory_allowed);
+  cudaError_t e = allow_shared_memory(paged_decode_kernel, smem_bytes(kHeads), &shared_memory_allowed);
   if (e != cudaSuccess) return e;
   const size_t rows = static_cast<size_t>(c.sequences) * q_heads * kRecord;
   SharedKeys shared = shared_keys_plan(c, q_heads);
@@ -406,8 +420,8 @@ cudaError_t launch_shared_prefix(const PagedCache& c, const void* q, const void*
   e = launch_shared_keys(c, q, k_pages, v_pages, q_heads, shared, stream);
   if (e != cudaSuccess) return e;
   // the sequences' own keys: nothing of it waits for the kernel before, so its CTAs start as that one's end
-  const int grid = decode_grid(c);
-  e = launch_pdl(paged_decode_kernel, dim3(grid), dim3(kThreads), kSmem, stream, a);
+  const int grid = decode_grid(c, q_heads);
+  e = launch_pdl(paged_decode_kernel, dim3(grid), dim3(kThreads), smem_bytes(q_heads / c.kv_heads), stream, a);
   if (e != cudaSuccess) return e;
   return launch_pdl(shared_prefix_merge_kernel, merge_grid(c, q_heads), dim3(kThreads), 0, stream, a, shared);
 }

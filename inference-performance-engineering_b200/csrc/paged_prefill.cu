@@ -179,25 +179,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_longer(bar, parity, err);
 }
 
-// Pairs of fp32 in one 64-bit register: two operations per instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float* lo, float* hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(*lo), "=f"(*hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // the largest of three; NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
