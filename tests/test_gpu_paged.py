@@ -262,6 +262,9 @@ PREFILL = [
     ([4] * 60, [n * 7 for n in range(60)], 16, 32, 8, 0),
     ([40], [30000], 32, 16, 8, 0),
     ([1500, 3], [0, 11], 16, 2, 2, 0),
+    ([(37 * n) % 211 for n in range(40)], [(91 * n) % 517 for n in range(40)], 16, 24, 8, 2),  # whole blocks, many per CTA
+    ([700, 1, 900, 40], [0, 3000, 100, 1], 128, 64, 8, 0),
+    ([n % 3 for n in range(1100)], [n % 5 for n in range(1100)], 16, 8, 8, 0),  # more sequences than are listed at once
 ]
 
 
@@ -316,6 +319,25 @@ def test_later_positions_do_not_reach_earlier_rows(bad):
     assert nat.device_error() == 0
 
 
+@pytest.mark.parametrize("bad", [NAN, float("inf")])
+def test_later_positions_beside_many_other_sequences(bad):
+    """The same where blocks stay whole, and every other sequence as it was."""
+    new = [150] * 40
+    b = Batch(new, [20] * 40, 16, 8, seed=19).fill(700)
+    q = normal((b.tokens, 8, 128), 20)
+    o, a = attend(b, q)
+    for s in (0, 17):
+        pages, rows = b.places(s, start=100)
+        b.v[pages, :, rows] = bad
+    out = prefill(b, q)
+    close = ((out.double() - o).abs() <= HALF * o.abs() + (HALF + 2.0 ** -11) * a).all(-1).view(40, 150)
+    sees = torch.zeros(40, 150, dtype=torch.bool, device=DEV)
+    sees[0, 80:] = sees[17, 80:] = True
+    assert torch.equal(close, ~sees)
+    assert not torch.isfinite(out.view(40, 150, -1)[sees]).any()
+    assert nat.device_error() == 0
+
+
 # ------------------------------------------------------------------------------------------ shared
 
 SHARED = [
@@ -329,6 +351,8 @@ SHARED = [
     ([8200, 8193], 64, 128, 12, 2),
     ([2048 + 13 * n for n in range(64)], 64, 32, 28, 4),
     ([1024] * 33, 32, 32, 32, 8),
+    ([33 + n % 40 for n in range(700)], 2, 16, 64, 8),  # more blocks of rows than CTAs
+    ([2600 + n for n in range(5)], 81, 32, 14, 2),
 ]
 
 
@@ -340,6 +364,20 @@ def test_shared_prefix(lengths, prefix, page, q_heads, kv_heads):
     check(out, b, q)
     assert torch.equal(out, shared(b, q))
     assert (out[b.lengths == 0] == 0).all()
+
+
+@pytest.mark.parametrize("bad", [NAN, float("inf"), torch.finfo(torch.bfloat16).min])
+def test_shared_keys_behind_a_rows_end(bad):
+    """A sequence that ends inside the prefix sees nothing of the prefix's later keys, whatever they hold."""
+    b = Batch([1] * 4, [39, 70, 150, 129], 16, 2, seed=27, prefix=12).fill(950)
+    q = normal((4, 8, 128), 28, 1.5)
+    o, a = attend(b, q)
+    pages, rows = b.places(0, count=192, start=151)
+    b.v[pages, :, rows] = bad
+    b.k[pages, 1:, rows] = bad
+    out = shared(b, q)
+    assert ((out.double() - o).abs() <= HALF * o.abs() + (HALF + 2.0 ** -11) * a).all()
+    assert nat.device_error() == 0
 
 
 def test_shared_prefix_is_paged_decode_on_whole_tables():

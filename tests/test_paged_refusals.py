@@ -12,6 +12,15 @@ GOOD = {
                                           table_dtype=0, table_rows=64, cu_tokens=16, lengths=16, page_table=16, sequences=2,
                                           max_pages=4, q_out=16, k_pages=16, v_pages=16, num_pages=9, page_size=16, eps=1e-6,
                                           stream=None),
+    "ipe_paged_decode_attention": dict(q=16, k_pages=16, v_pages=16, page_table=16, lengths=16, out=16, sequences=2,
+                                       q_heads=16, kv_heads=8, num_pages=9, page_size=16, max_pages=4, workspace=256,
+                                       workspace_bytes=1 << 30, stream=None),
+    "ipe_paged_prefill_attention": dict(q=16, k_pages=16, v_pages=16, page_table=16, cu_tokens=16, lengths=16, out=16,
+                                        tokens=5, sequences=2, q_heads=16, kv_heads=8, num_pages=9, page_size=16,
+                                        max_pages=4, workspace=256, workspace_bytes=1 << 30, stream=None),
+    "ipe_shared_prefix_attention": dict(q=16, k_pages=16, v_pages=16, prefix_pages=16, prefix_count=2, page_table=16,
+                                        lengths=16, out=16, sequences=2, q_heads=16, kv_heads=8, num_pages=9, page_size=16,
+                                        max_pages=4, workspace=256, workspace_bytes=1 << 30, stream=None),
 }
 
 BAD = [
@@ -31,7 +40,26 @@ BAD = [
     ("ipe_paged_qk_norm_rope_append", dict(table_rows=0)),
 ] + [("ipe_paged_qk_norm_rope_append", {p: v}) for p in
      ("qkv", "q_norm", "k_norm", "cos", "sin", "cu_tokens", "lengths", "page_table", "q_out", "k_pages", "v_pages")
-     for v in (None, 18)]
+     for v in (None, 18)] + [
+    (name, change)
+    for name in ("ipe_paged_decode_attention", "ipe_paged_prefill_attention", "ipe_shared_prefix_attention")
+    for change in [dict(q_heads=15), dict(q_heads=72), dict(q_heads=0), dict(kv_heads=0), dict(page_size=8), dict(page_size=48),
+                   dict(num_pages=0), dict(num_pages=2 ** 25), dict(max_pages=0), dict(max_pages=2 ** 24),
+                   dict(sequences=-1), dict(sequences=2 ** 25), dict(workspace=None), dict(workspace=16),
+                   dict(workspace_bytes=64)] +
+                  [{p: v} for p in ("q", "k_pages", "v_pages", "page_table", "lengths", "out") for v in (None, 18)]] + [
+    ("ipe_paged_prefill_attention", dict(tokens=-1)),
+    ("ipe_paged_prefill_attention", dict(tokens=2 ** 28)),
+    ("ipe_paged_prefill_attention", dict(cu_tokens=None)),
+    ("ipe_paged_prefill_attention", dict(cu_tokens=17)),
+    ("ipe_shared_prefix_attention", dict(prefix_count=-1)),
+    ("ipe_shared_prefix_attention", dict(prefix_count=5)),
+    ("ipe_shared_prefix_attention", dict(prefix_pages=None)),
+    ("ipe_shared_prefix_attention", dict(prefix_pages=18)),
+    ("ipe_shared_prefix_attention", dict(sequences=2 ** 22, prefix_count=2 ** 11, max_pages=2 ** 11)),
+    # units of 64 keys past 32 bits
+    ("ipe_paged_decode_attention", dict(sequences=2 ** 20, max_pages=2 ** 20)),
+]
 
 
 @pytest.mark.parametrize(("name", "change"), BAD)
@@ -42,9 +70,23 @@ def test_the_entry_points_refuse(name, change):
 
 
 def test_nothing_to_do_is_no_error():
-    name = "ipe_paged_qk_norm_rope_append"
-    for change in (dict(tokens=0, qkv=None, q_out=None), dict(sequences=0, page_table=None)):
+    for name, change in [("ipe_paged_qk_norm_rope_append", dict(tokens=0, qkv=None, q_out=None)),
+                         ("ipe_paged_qk_norm_rope_append", dict(sequences=0, page_table=None)),
+                         ("ipe_paged_decode_attention", dict(sequences=0, q=None, out=None, page_table=None, workspace=None)),
+                         ("ipe_paged_prefill_attention", dict(tokens=0, q=None, out=None, workspace=None)),
+                         ("ipe_shared_prefix_attention", dict(sequences=0, q=None, out=None, lengths=None))]:
         assert getattr(nat.load(), name)(*{**GOOD[name], **change}.values()) == 0
+
+
+def test_the_workspaces_sizes():
+    """Nothing for sizes that make no call; what splits work needs room, and more where there are more parts."""
+    lib = nat.load()
+    assert lib.ipe_paged_decode_attention_workspace(0, 16, 8) == 0
+    assert lib.ipe_paged_decode_attention_workspace(4, 40, 8) > lib.ipe_paged_decode_attention_workspace(4, 16, 8) > 0
+    assert lib.ipe_paged_prefill_attention_workspace(0, 1, 16, 8) == 0
+    assert lib.ipe_paged_prefill_attention_workspace(100, 1, 16, 8) > 0
+    assert lib.ipe_paged_prefill_attention_workspace(100000, 1, 16, 8) == 0  # whole blocks: no parts
+    assert lib.ipe_shared_prefix_attention_workspace(4, 16, 8, 16, 9) > lib.ipe_paged_decode_attention_workspace(4, 16, 8)
 
 
 def test_cpu_tensors_are_refused():
