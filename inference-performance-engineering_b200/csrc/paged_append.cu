@@ -95,6 +95,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const int slot0 = warp % split * share, width = min(slots, slot0 + share) - slot0;  // of the slots
   const int rows = mine > 0 && width > 0 ? mine * width : 0;  // one run: several tokens only with all their slots
   if (rows == 0) return;
+  pdl_wait();  // for the kernels that wrote qkv, or still read what is written here
+  pdl_trigger();
   unsigned char* ring = smem + local * (kStages * kPiece * 256);
   const bf16* src = qkv + (static_cast<int64_t>(t0) * slots + slot0) * 128;
   auto fetch = [&](int piece) {
@@ -219,12 +221,10 @@ cudaError_t launch_paged_append(const PagedCache& c, const void* qkv, int64_t to
                               : allow_shared_memory(paged_append_kernel<bf16>, kSmem, &allowed[0]);
   if (e != cudaSuccess) return e;
   if (fp32_tables)
-    paged_append_kernel<float><<<grid, kThreads, kSmem, stream>>>(c, x, n, per_warp, split, q_heads, qn, kn, static_cast<const float*>(cos_t),
-                                                              static_cast<const float*>(sin_t), table_rows, q, k, v, eps);
-  else
-    paged_append_kernel<bf16><<<grid, kThreads, kSmem, stream>>>(c, x, n, per_warp, split, q_heads, qn, kn, static_cast<const bf16*>(cos_t),
-                                                             static_cast<const bf16*>(sin_t), table_rows, q, k, v, eps);
-  return cudaGetLastError();
+    return launch_pdl(paged_append_kernel<float>, dim3(grid), dim3(kThreads), kSmem, stream, c, x, n, per_warp, split, q_heads,
+                      qn, kn, static_cast<const float*>(cos_t), static_cast<const float*>(sin_t), table_rows, q, k, v, eps);
+  return launch_pdl(paged_append_kernel<bf16>, dim3(grid), dim3(kThreads), kSmem, stream, c, x, n, per_warp, split, q_heads,
+                    qn, kn, static_cast<const bf16*>(cos_t), static_cast<const bf16*>(sin_t), table_rows, q, k, v, eps);
 }
 
 }  // namespace ipe

@@ -86,6 +86,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
   const PagedCache& c = a.c;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.q_heads / c.kv_heads;
+  // Behind the kernel of the shared keys, which starts when the kernels before it have finished, this one starts
+  // early and has nothing to wait for.
   pdl_trigger();
 
   // ------------------------------------------------------------------ this CTA's run of units

@@ -212,14 +212,14 @@ __device__ __forceinline__ void exp2_pair(uint64_t x, float* p0, float* p1) {
 __device__ __forceinline__ void attend_row(const PagedCache& c, const bf16* q_row, const bf16* k, const bf16* v, int s,
                                         int kv_head, int from, int to, float* o, float* top, float* sum) {
   const int lane = threadIdx.x & 31;
-  const uint2 raw = *reinterpret_cast<const uint2*>(q_row + lane * 4);
+  const uint2 raw = ldcg8(q_row + lane * 4);
   const float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
                       __uint_as_float(raw.y & 0xffff0000u)};
   float m = -INFINITY, l = 0.f;
   o[0] = o[1] = o[2] = o[3] = 0.f;
   for (int key = from; key < to; ++key) {
     const int64_t at = (c.page_row(c.page(s, key), kv_head) + (key & (c.page_size() - 1))) * 128 + lane * 4;
-    const uint2 kr = *reinterpret_cast<const uint2*>(k + at), vr = *reinterpret_cast<const uint2*>(v + at);
+    const uint2 kr = ldcg8(k + at), vr = ldcg8(v + at);
     float dot = x[0] * __uint_as_float(kr.x << 16) + x[1] * __uint_as_float(kr.x & 0xffff0000u) +
                 x[2] * __uint_as_float(kr.y << 16) + x[3] * __uint_as_float(kr.y & 0xffff0000u);
     dot = warp_sum(dot);
@@ -863,30 +863,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The blocks whose key tiles lie in more than one run: a CTA per (block, KV head, 16 rows), a warp per row at
-// a time.
-constexpr int kMergeRows = 16;
-__global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
+// The blocks whose key tiles lie in more than one run: a CTA per (block, KV head, 8 rows), a warp per row.
+constexpr int kMergeRows = 8;
+__global__ void __launch_bounds__(kMergeRows * 32) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
   const int block = blockIdx.x / a.c.kv_heads, kv_head = blockIdx.x - block * a.c.kv_heads;
   const int group = a.q_heads / a.c.kv_heads, per_tile = kBM / group;
   pdl_wait();
-  if (block >= min(__ldcg(&a.blocks[-1].x), a.most_blocks)) return;
+  const int blocks = min(__ldcg(&a.blocks[-1].x), a.most_blocks);  // loaded together; of a block that is none, nothing is used
   const int2 item = __ldcg(a.items + blockIdx.x);
-  // whole, already written; or what a kernel that gave up on a wait left
-  if (item.x < 0 || item.y >= ctas || item.y < item.x >> 1) return;
   const int4 b = __ldcg(a.blocks + block);
-  for (int k = threadIdx.x >> 5; k < kMergeRows; k += 8) {
-    const int r = blockIdx.y * kMergeRows + k, tile = r / kBM, in_tile = r - tile * kBM;
-    const int place = in_tile / group, token = tile * per_tile + place;
-    if (place >= per_tile || token >= b.y || b.x < 0 || b.x + token >= a.tokens) continue;
-    bf16* row = a.out + (static_cast<int64_t>(b.x + token) * a.q_heads + kv_head * group + in_tile - place * group) * 128;
-    Parts parts[1];
-    parts[0].blocks(a.records, r, item);
-    if (b.z + token < 0)  // no position: no keys
-      *reinterpret_cast<uint2*>(row + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
-    else
-      join_parts(parts, row);
-  }
+  // whole, already written; or what a kernel that gave up on a wait left
+  if (block >= blocks || item.x < 0 || item.y >= ctas || item.y < item.x >> 1) return;
+  const int r = blockIdx.y * kMergeRows + (threadIdx.x >> 5), tile = r / kBM, in_tile = r - tile * kBM;
+  const int place = in_tile / group, token = tile * per_tile + place;
+  if (place >= per_tile || token >= b.y || b.x < 0 || b.x + token >= a.tokens) return;
+  bf16* row = a.out + (static_cast<int64_t>(b.x + token) * a.q_heads + kv_head * group + in_tile - place * group) * 128;
+  Parts parts[1];
+  parts[0].blocks(a.records, r, item);
+  if (b.z + token < 0)  // no position: no keys
+    *reinterpret_cast<uint2*>(row + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
+  else
+    join_parts(parts, row);
 }
 
 // most blocks that `tokens` new tokens of `sequences` sequences make
@@ -969,7 +966,7 @@ cudaError_t launch_paged_prefill(const PagedCache& c, const void* q, const void*
   e = launch<false>(grid, maps, a, stream);
   if (e != cudaSuccess || !in_runs) return e;
   return launch_pdl(paged_prefill_merge_kernel, dim3(static_cast<unsigned>(blocks * c.kv_heads), 2 * kBM / kMergeRows),
-                    dim3(256), 0, stream, a, static_cast<int>(grid));
+                    dim3(kMergeRows * 32), 0, stream, a, static_cast<int>(grid));
 }
 
 SharedKeys shared_keys_plan(const PagedCache& c, int q_heads) {

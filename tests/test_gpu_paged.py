@@ -469,6 +469,37 @@ def test_replays_with_other_lengths_and_tables():
             check(out, b, q)
 
 
+def test_a_captured_step_behind_copies_and_fills():
+    """The operators' kernels start early behind other kernels; behind copies and fills, captured too, they read what
+    those wrote."""
+    b = Batch([1] * 3, [100, 60, 200], 16, 2, seed=42).fill(1150)
+    q_new = normal((3, 4, 128), 43)
+    q, out = torch.zeros_like(q_new), torch.zeros(3, 512, dtype=torch.bfloat16, device=DEV)
+    lengths_new = b.lengths.clone()
+
+    def step():
+        b.lengths.zero_()
+        ops.paged_decode_attention(q, b.k, b.v, b.page_table, b.lengths, out)
+        b.lengths.copy_(lengths_new)
+        q.copy_(q_new)
+        ops.paged_decode_attention(q, b.k, b.v, b.page_table, b.lengths, out)
+        out_first.copy_(out)
+        ops.paged_prefill_attention(q, b.k, b.v, b.page_table, b.cu, b.lengths, out)
+
+    out_first = torch.zeros_like(out)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for round_ in range(3):
+        q_new.copy_(normal(q_new.shape, 44 + round_))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out_first, b, q_new)
+        check(out, b, q_new)
+
+
 def test_calls_on_two_streams_at_once():
     batches = [Batch([1] * 5, [700 + 90 * n + s for n in range(5)], 32, 2, seed=50 + s, prefix=10).fill(1200 + 50 * s) for s in range(2)]
     queries = [normal((5, 8, 128), 60 + s) for s in range(2)]
