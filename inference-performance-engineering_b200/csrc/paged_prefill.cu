@@ -349,167 +349,200 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   if (threadIdx.x == 0 && sh.tmem != kTmem) report(err, kErrShape);
   if (warp >= kLoadWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == kLoadWarp) {
-    // ------------------------------------------------------------------ work list and loads
-    if (lane < 3)
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v))
-                   : "memory");
-    const int ps = c.page_size(), subs = kBN >> c.page_shift;
-    // In runs: sh.low = blocks before each sequence, sh.high = key tiles before each block. Otherwise
-    // sh.low .. sh.high: the sequence's blocks as numbers that grow with their keys (block 0 of a sequence
-    // on a context starts at the context's length in blocks), `most` past the largest.
-    const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
-    int blocks = 0, tiles = 0, most = 0;
-    bool whole = false;
-    if (kShared) {
-      blocks = (a.tokens + per_block - 1) / per_block;
-      tiles = blocks * shared_tiles;
-    } else {
-      for (int base = 0; base < c.sequences; base += 32) {
-        const int s = base + lane;
-        Span x{0, 0, 0};
-        if (s < c.sequences) x = span_of(c, s, a.tokens);
-        const int n = (x.tokens + per_block - 1) / per_block, first = max(0, x.length - x.tokens) / per_block;
-        const int before = blocks + warp_scan(n);
-        if (s < kMaxListed) {
-          sh.low[s] = in_runs ? min(before, a.most_blocks) : first;
-          sh.high[s] = first + n;
-        }
-        if (n > 0) most = max(most, first + n);
-        blocks = __shfl_sync(0xffffffffu, before + n, 31);
-      }
-      most = __reduce_max_sync(0xffffffffu, most);
-      __syncwarp();
-    }
-    if (!kShared && in_runs) {
-      blocks = min(blocks, a.most_blocks);
-      if (blockIdx.x == 0 && lane == 0) a.blocks[-1].x = blocks;
-      int longest = 0;
-      for (int base = 0; base < blocks; base += 32) {
-        const int i = base + lane;
-        int n = 0;
-        if (i < blocks) {
-          const int s = last_at_most(sh.low, c.sequences, i);
-          n = tiles_of(block_keys(span_of(c, s, a.tokens), i - sh.low[s], per_block));
-        }
-        const int before = tiles + warp_scan(n);
-        if (i < blocks) sh.high[i] = before;
-        longest = max(longest, n);
-        tiles = __shfl_sync(0xffffffffu, before + n, 31);
-      }
-      // Whole blocks after all where the runs would save less than the records and their merge cost, which
-      // is the time of about 5 key tiles (9 us).
-      longest = __reduce_max_sync(0xffffffffu, longest);
-      const int ctas = gridDim.x;
-      whole = longest * ((blocks * c.kv_heads + ctas - 1) / ctas) <= (tiles * c.kv_heads + ctas - 1) / ctas + 5;
-      if (whole) {
-        for (int i = lane; i < blocks; i += 32) sh.high[i] = i;  // a block is one unit
-        tiles = blocks;
-      }
-      if (lane == 0) sh.high[blocks] = tiles;
-      __syncwarp();
-    }
-    const int works = blocks * c.kv_heads;
-    const Deal deal(in_runs ? tiles * c.kv_heads : 0, gridDim.x);
-    int unit = deal.start(blockIdx.x);  // in runs
-    const int unit_end = deal.start(blockIdx.x + 1);
-    const bool listed = c.sequences <= kMaxListed;
-    auto range_of = [&](int s, int* low, int* high) {
-      if (listed) {
-        *low = sh.low[s];
-        *high = sh.high[s];
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp) {
+      // ------------------------------------------------------------------ work list and loads
+      if (lane < 3)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v))
+                     : "memory");
+      const int ps = c.page_size(), subs = kBN >> c.page_shift;
+      // In runs: sh.low = blocks before each sequence, sh.high = key tiles before each block. Otherwise
+      // sh.low .. sh.high: the sequence's blocks as numbers that grow with their keys (block 0 of a sequence
+      // on a context starts at the context's length in blocks), `most` past the largest.
+      const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
+      int blocks = 0, tiles = 0, most = 0;
+      bool whole = false;
+      if (kShared) {
+        blocks = (a.tokens + per_block - 1) / per_block;
+        tiles = blocks * shared_tiles;
       } else {
-        const Span x = span_of(c, s, a.tokens);
-        *low = max(0, x.length - x.tokens) / per_block;
-        *high = *low + (x.tokens + per_block - 1) / per_block;
-      }
-    };
-    // the `rank`-th block in descending order of its number; the whole warp takes part
-    auto select = [&](int rank, int* seq, int* block) {
-      auto at_least = [&](int x) {
-        int n = 0;
-        for (int s = lane; s < c.sequences; s += 32) {
-          int low, high;
-          range_of(s, &low, &high);
-          n += max(0, high - max(low, x));
+        for (int base = 0; base < c.sequences; base += 32) {
+          const int s = base + lane;
+          Span x{0, 0, 0};
+          if (s < c.sequences) x = span_of(c, s, a.tokens);
+          const int n = (x.tokens + per_block - 1) / per_block, first = max(0, x.length - x.tokens) / per_block;
+          const int before = blocks + warp_scan(n);
+          if (s < kMaxListed) {
+            sh.low[s] = in_runs ? min(before, a.most_blocks) : first;
+            sh.high[s] = first + n;
+          }
+          if (n > 0) most = max(most, first + n);
+          blocks = __shfl_sync(0xffffffffu, before + n, 31);
         }
-        return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
-      };
-      int lo = 0, hi = most;  // at_least(lo) > rank >= at_least(hi)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (at_least(mid) > rank) lo = mid;
-        else hi = mid;
+        most = __reduce_max_sync(0xffffffffu, most);
+        __syncwarp();
       }
-      int left = rank - at_least(lo + 1);  // so many sequences with a block `lo` come before
-      for (int base = 0; base < c.sequences; base += 32) {
-        const int s = base + lane;
-        int low = 0, high = 0;
-        if (s < c.sequences) range_of(s, &low, &high);
-        const unsigned has = __ballot_sync(0xffffffffu, s < c.sequences && low <= lo && lo < high);
-        const int n = __popc(has);
-        if (left < n) {
-          const int at = __fns(has, 0, left + 1);
-          *seq = base + at;
-          *block = lo - __shfl_sync(0xffffffffu, low, at);
-          return;
+      if (!kShared && in_runs) {
+        blocks = min(blocks, a.most_blocks);
+        if (blockIdx.x == 0 && lane == 0) a.blocks[-1].x = blocks;
+        int longest = 0;
+        for (int base = 0; base < blocks; base += 32) {
+          const int i = base + lane;
+          int n = 0;
+          if (i < blocks) {
+            const int s = last_at_most(sh.low, c.sequences, i);
+            n = tiles_of(block_keys(span_of(c, s, a.tokens), i - sh.low[s], per_block));
+          }
+          const int before = tiles + warp_scan(n);
+          if (i < blocks) sh.high[i] = before;
+          longest = max(longest, n);
+          tiles = __shfl_sync(0xffffffffu, before + n, 31);
         }
-        left -= n;
+        // Whole blocks after all where the runs would save less than the records and their merge cost, which
+        // is the time of about 5 key tiles (9 us).
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        const int ctas = gridDim.x;
+        whole = longest * ((blocks * c.kv_heads + ctas - 1) / ctas) <= (tiles * c.kv_heads + ctas - 1) / ctas + 5;
+        if (whole) {
+          for (int i = lane; i < blocks; i += 32) sh.high[i] = i;  // a block is one unit
+          tiles = blocks;
+        }
+        if (lane == 0) sh.high[blocks] = tiles;
+        __syncwarp();
       }
-      *seq = 0;
-      *block = 0;
-    };
-
-    int slot = 0, piece = 0;
-    uint32_t phase = 0, armed = 0;  // bit s: parity armed on pair_full[s]; bit 16 + s: armed at all
-    bool ok = true;
-    for (int round = 0; ok && !*abort_flag; ++round, ++piece) {
-      Work w;
-      if (in_runs) {
-        if (unit >= unit_end) break;
-        const int block = kShared ? unit / (shared_tiles * c.kv_heads) : last_at_most(sh.high, blocks, unit / c.kv_heads);
-        const int before = kShared ? block * shared_tiles : sh.high[block];
-        const int n = kShared ? shared_tiles : sh.high[block + 1] - before;
-        const int r = unit - before * c.kv_heads, kv_head = r / n;
-        const int tile0 = r - kv_head * n, tile1 = min(n, tile0 + unit_end - unit);
-        if (tile0 == 0 && lane == 0)
-          a.items[static_cast<int64_t>(block) * c.kv_heads + kv_head] = item_parts(deal, unit, n, blockIdx.x);
-        if (kShared) {
-          // every row sees up to all shared keys: as if the tokens stood behind them
-          w = make_work(Span{0, a.tokens, a.shared_keys + a.tokens}, 0, block, kv_head, per_tile, tile0, tile1);
-          w.keys = a.shared_keys;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) w.count[i] = w.tokens > i * per_tile ? tile1 - tile0 : 0;
+      const int works = blocks * c.kv_heads;
+      const Deal deal(in_runs ? tiles * c.kv_heads : 0, gridDim.x);
+      int unit = deal.start(blockIdx.x);  // in runs
+      const int unit_end = deal.start(blockIdx.x + 1);
+      const bool listed = c.sequences <= kMaxListed;
+      auto range_of = [&](int s, int* low, int* high) {
+        *low = *high = 0;
+        if (s >= c.sequences) return;
+        if (listed) {
+          *low = sh.low[s];
+          *high = sh.high[s];
         } else {
-          const int s = last_at_most(sh.low, c.sequences, block);
-          w = make_work(span_of(c, s, a.tokens), s, block - sh.low[s], kv_head, per_tile, tile0, whole ? -1 : tile1);
-          if (tile0 == 0 && kv_head == 0 && lane == 0) a.blocks[block] = make_int4(w.token0, w.tokens, w.position0, 0);
+          const Span x = span_of(c, s, a.tokens);
+          *low = max(0, x.length - x.tokens) / per_block;
+          *high = *low + (x.tokens + per_block - 1) / per_block;
         }
-        if (tile0 > 0 || tile1 < n) w.record = static_cast<int>(blockIdx.x) * 2 + (round == 0 ? 0 : 1);
-        unit += tile1 - tile0;
-      } else {
-        const int ctas = gridDim.x, turn = round * ctas;
-        const int rank = turn + ((round & 1) ? ctas - 1 - blockIdx.x : blockIdx.x);
-        if (turn >= works) break;
-        if (rank >= works) {
-          --piece;  // nothing this round; the next one is empty
-          continue;
+      };
+      // the `rank`-th block in descending order of its number; the whole warp takes part
+      int low0, high0;
+      range_of(lane, &low0, &high0);
+      auto select = [&](int rank, int* seq, int* block) {
+        auto at_least = [&](int x) {
+          int n = max(0, high0 - max(low0, x));
+          for (int s = lane + 32; s < c.sequences; s += 32) {
+            int low, high;
+            range_of(s, &low, &high);
+            n += max(0, high - max(low, x));
+          }
+          return static_cast<int>(__reduce_add_sync(0xffffffffu, n));
+        };
+        int lo = 0, hi = most, above = 0;  // at_least(lo) > rank >= at_least(hi) = above
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1, n = at_least(mid);
+          if (n > rank) {
+            lo = mid;
+          } else {
+            hi = mid;
+            above = n;
+          }
         }
-        int s, b;
-        select(rank / c.kv_heads, &s, &b);
-        w = make_work(span_of(c, s, a.tokens), s, b, rank % c.kv_heads, per_tile, 0, -1);
-      }
-      const int steps = max(w.count[0], w.count[1]);
+        int left = rank - above;  // so many sequences with a block `lo` come before
+        *seq = *block = 0;
+        for (int base = 0; base < c.sequences; base += 32) {
+          int low = low0, high = high0;
+          if (base > 0) range_of(base + lane, &low, &high);
+          const bool has = low <= lo && lo < high;
+          const unsigned all = __ballot_sync(0xffffffffu, has);
+          const unsigned it = __ballot_sync(0xffffffffu, has && __popc(all & ((1u << lane) - 1)) == left);
+          if (it != 0) {
+            const int at = __ffs(it) - 1;
+            *seq = base + at;
+            *block = lo - __shfl_sync(0xffffffffu, low, at);
+            return;
+          }
+          left -= __popc(all);
+        }
+      };
+      // The next piece of this CTA's list, if there is one.
+      int round = 0;
+      auto take = [&](Work* out) {
+        Work w;
+        if (in_runs) {
+          if (unit >= unit_end) return false;
+          const int block = kShared ? unit / (shared_tiles * c.kv_heads) : last_at_most(sh.high, blocks, unit / c.kv_heads);
+          const int before = kShared ? block * shared_tiles : sh.high[block];
+          const int n = kShared ? shared_tiles : sh.high[block + 1] - before;
+          const int r = unit - before * c.kv_heads, kv_head = r / n;
+          const int tile0 = r - kv_head * n, tile1 = min(n, tile0 + unit_end - unit);
+          if (tile0 == 0 && lane == 0)
+            a.items[static_cast<int64_t>(block) * c.kv_heads + kv_head] = item_parts(deal, unit, n, blockIdx.x);
+          if (kShared) {
+            // every row sees up to all shared keys: as if the tokens stood behind them
+            w = make_work(Span{0, a.tokens, a.shared_keys + a.tokens}, 0, block, kv_head, per_tile, tile0, tile1);
+            w.keys = a.shared_keys;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w.count[i] = w.tokens > i * per_tile ? tile1 - tile0 : 0;
+          } else {
+            const int s = last_at_most(sh.low, c.sequences, block);
+            w = make_work(span_of(c, s, a.tokens), s, block - sh.low[s], kv_head, per_tile, tile0, whole ? -1 : tile1);
+            if (tile0 == 0 && kv_head == 0 && lane == 0) a.blocks[block] = make_int4(w.token0, w.tokens, w.position0, 0);
+          }
+          if (tile0 > 0 || tile1 < n) w.record = static_cast<int>(blockIdx.x) * 2 + (round == 0 ? 0 : 1);
+          unit += tile1 - tile0;
+          ++round;
+        } else {
+          const int ctas = gridDim.x;
+          int rank;
+          do {  // a round that ends before this CTA's place is the last one but for an empty one
+            if (round * ctas >= works) return false;
+            rank = round * ctas + ((round & 1) ? ctas - 1 - blockIdx.x : blockIdx.x);
+            ++round;
+          } while (rank >= works);
+          int s, b;
+          select(rank / c.kv_heads, &s, &b);
+          w = make_work(span_of(c, s, a.tokens), s, b, rank % c.kv_heads, per_tile, 0, -1);
+        }
+        *out = w;
+        return true;
+      };
+
+      // One pair of tiles at a time. The next piece is looked up while the one at hand has its first pairs on
+      // their way: that takes about two steps' time (7000 cycles with its loads), which nobody then waits for.
+      int slot = 0, piece = 0, step = 0, steps = -1;
+      uint32_t phase = 0, armed = 0;  // bit s: parity armed on pair_full[s]; bit 16 + s: armed at all
+      bool ok = true, known = false, more = false;
+      Work w, next;
       // This lane's page of a step's tile: its ID is loaded a step ahead and looked at when it is used.
-      auto key_of = [&](int step) { return (w.tile0 + step) * kBN + lane * ps; };
-      auto has_page = [&](int step) { return lane < subs && step < steps && key_of(step) < w.keys; };
-      auto load_id = [&](int step) { return has_page(step) ? c.page_id(w.sequence, key_of(step)) : 0; };
-      int id = load_id(0), row = 0, row_v = 0;  // cache rows of the keys to load, and of the step before
-      bool has = has_page(0), has_v = false;
-      for (int step = 0; step <= steps; ++step) {  // keys of `step`, values of the step before
+      auto key_of = [&](const Work& x, int step) { return (x.tile0 + step) * kBN + lane * ps; };
+      auto has_page = [&](const Work& x, int step) {
+        return lane < subs && step < max(x.count[0], x.count[1]) && key_of(x, step) < x.keys;
+      };
+      auto load_id = [&](const Work& x, int step) { return has_page(x, step) ? c.page_id(x.sequence, key_of(x, step)) : 0; };
+      int id = 0, id_next = 0, row = 0, row_v = 0;  // cache rows of the keys to load, and of the step before
+      bool has = false, has_v = false;
+      while (!*abort_flag) {
+        if (!known && (step > steps || step == 3)) {
+          known = true;
+          more = take(&next);
+          if (more) id_next = load_id(next, 0);
+        }
+        if (step > steps) {
+          if (!more) break;
+          w = next;
+          id = id_next;
+          known = false;
+          step = 0;
+          steps = max(w.count[0], w.count[1]);
+          has = has_page(w, 0);
+          has_v = false;
+        }
+        // keys of `step`, values of the step before
         if (has) row = static_cast<int>(c.page_row(c.checked(id), w.kv_head));
-        id = load_id(step + 1);
+        id = load_id(w, step + 1);
         const int parts = __popc(__ballot_sync(0xffffffffu, has)) + __popc(__ballot_sync(0xffffffffu, has_v));
         if (!wait_warp(&sh.pair_empty[slot], phase ^ 1, err)) {
           ok = false;
@@ -544,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           __syncwarp();
+          ++piece;
         }
         if (++slot == kStages) {
           slot = 0;
@@ -551,122 +585,121 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         row_v = row;
         has_v = has;
-        has = has_page(step + 1);
+        has = has_page(w, ++step);
       }
-    }
-    if (!ok) *abort_flag = 1;
-    // tell the others that the list has ended
-    if (ok && !*abort_flag && wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
-      if (lane == 0) {
-        sh.work[piece & 1].token0 = -1;
-        mbar_arrive(&sh.q_full);
-      }
-    } else {
-      *abort_flag = 1;
-    }
-    // copies and arrivals in flight land before the CTA's shared memory goes away
-    for (int s = 0; s < kStages; ++s) {
-      if (!(armed & (1u << (16 + s)))) continue;
-      mbar_wait(&sh.pair_full[s], (armed >> s) & 1u, err);
-      if (!*abort_flag) mbar_wait(&sh.pair_empty[s], (armed >> s) & 1u, err);
-    }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------------ MMA issue
-    // Everything an MMA is given is the same in all lanes and looks so to the compiler (constants, loop
-    // counters, warp reductions): operands that may differ cost it about 100 cycles per MMA.
-    constexpr uint32_t idesc_s = instr_desc(false), idesc_o = instr_desc(true);
-    const uint32_t q_desc = desc_kmajor(smem_addr(s_q)), k_desc = desc_kmajor(smem_addr(ring) + kTile),
-                   v_desc = desc_mnmajor(smem_addr(ring));
-    uint32_t it = 0;  // pairs taken so far
-    uint32_t p_seen[2] = {0, 0}, o_seen[2] = {0, 0};
-    auto wait_pair = [&] { return wait_warp(&sh.pair_full[it % kStages], (it / kStages) & 1, err); };
-    auto issue_s = [&](int i) {  // S_i = Q_i K^T
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t qd = q_desc + i * (kTile >> 4), kd = k_desc + (it % kStages) * (2 * kTile >> 4);
-#pragma unroll
-        for (uint32_t kk = 0; kk < kD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kHalf >> 4) + 2 * (kk & 3);  // 64-column half, 32 bytes per 16 columns
-          mma_smem(kTmem + i * kBN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+      if (!ok) *abort_flag = 1;
+      // tell the others that the list has ended
+      if (ok && !*abort_flag && wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
+        if (lane == 0) {
+          sh.work[piece & 1].token0 = -1;
+          mbar_arrive(&sh.q_full);
         }
-        mma_commit(&sh.s_full[i]);
+      } else {
+        *abort_flag = 1;
       }
-      __syncwarp();
-    };
-    auto issue_o = [&](int i, bool first, int half) {  // O_i (+)= P_i V over 64 keys
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t vd = v_desc + (it % kStages) * (2 * kTile >> 4);
+      // copies and arrivals in flight land before the CTA's shared memory goes away
+      for (int s = 0; s < kStages; ++s) {
+        if (!(armed & (1u << (16 + s)))) continue;
+        mbar_wait(&sh.pair_full[s], (armed >> s) & 1u, err);
+        if (!*abort_flag) mbar_wait(&sh.pair_empty[s], (armed >> s) & 1u, err);
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------------ MMA issue
+      // Everything an MMA is given is the same in all lanes and looks so to the compiler (constants, loop
+      // counters, warp reductions): operands that may differ cost it about 100 cycles per MMA.
+      constexpr uint32_t idesc_s = instr_desc(false), idesc_o = instr_desc(true);
+      const uint32_t q_desc = desc_kmajor(smem_addr(s_q)), k_desc = desc_kmajor(smem_addr(ring) + kTile),
+                     v_desc = desc_mnmajor(smem_addr(ring));
+      uint32_t it = 0;  // pairs taken so far
+      uint32_t p_seen[2] = {0, 0}, o_seen[2] = {0, 0};
+      auto wait_pair = [&] { return wait_warp(&sh.pair_full[it % kStages], (it / kStages) & 1, err); };
+      auto issue_s = [&](int i) {  // S_i = Q_i K^T
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t qd = q_desc + i * (kTile >> 4), kd = k_desc + (it % kStages) * (2 * kTile >> 4);
 #pragma unroll
-        for (uint32_t kk = half * 4; kk < half * 4 + 4; ++kk)
-          mma_tmem(kTmem + 256 + i * kBN, kTmem + i * kBN + kk * 8, vd + kk * (16 * 128 >> 4), idesc_o,
-                   (!first || kk > 0) ? 1u : 0u);
-      }
-      __syncwarp();
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (elect_one()) mma_commit(bar);
-      __syncwarp();
-    };
-    bool ok = true;
-    for (int piece = 0; ok && !*abort_flag; ++piece) {
-      if (!wait_warp(&sh.q_full, piece & 1, err)) {
-        ok = false;
-        break;
-      }
-      const int token0 = sh.work[piece & 1].token0, count0 = sh.work[piece & 1].count[0],
-                count1 = sh.work[piece & 1].count[1], left = sh.work[piece & 1].keys - sh.work[piece & 1].tile0 * kBN;
-      if (token0 < 0) break;
-      const int count[2] = {static_cast<int>(__reduce_max_sync(0xffffffffu, count0)),
-                            static_cast<int>(__reduce_max_sync(0xffffffffu, count1))};
-      const int steps = max(count[0], count[1]);
-      if (!wait_pair()) {
-        ok = false;
-        break;
-      }
+          for (uint32_t kk = 0; kk < kD / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kHalf >> 4) + 2 * (kk & 3);  // 64-column half, 32 bytes per 16 columns
+            mma_smem(kTmem + i * kBN, qd + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&sh.s_full[i]);
+        }
+        __syncwarp();
+      };
+      auto issue_o = [&](int i, bool first, int half) {  // O_i (+)= P_i V over 64 keys
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t vd = v_desc + (it % kStages) * (2 * kTile >> 4);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (count[i] > 0) issue_s(i);
-      commit(&sh.pair_empty[it % kStages]);
-      if (steps == 1) commit(&sh.q_empty);
-      ++it;
-      for (int step = 0; step < steps; ++step, ++it) {
+          for (uint32_t kk = half * 4; kk < half * 4 + 4; ++kk)
+            mma_tmem(kTmem + 256 + i * kBN, kTmem + i * kBN + kk * 8, vd + kk * (16 * 128 >> 4), idesc_o,
+                     (!first || kk > 0) ? 1u : 0u);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) mma_commit(bar);
+        __syncwarp();
+      };
+      bool ok = true;
+      for (int piece = 0; ok && !*abort_flag; ++piece) {
+        if (!wait_warp(&sh.q_full, piece & 1, err)) {
+          ok = false;
+          break;
+        }
+        const int token0 = sh.work[piece & 1].token0, count0 = sh.work[piece & 1].count[0],
+                  count1 = sh.work[piece & 1].count[1], left = sh.work[piece & 1].keys - sh.work[piece & 1].tile0 * kBN;
+        if (token0 < 0) break;
+        const int count[2] = {static_cast<int>(__reduce_max_sync(0xffffffffu, count0)),
+                              static_cast<int>(__reduce_max_sync(0xffffffffu, count1))};
+        const int steps = max(count[0], count[1]);
         if (!wait_pair()) {
           ok = false;
           break;
         }
-        const int valid = left - step * kBN;
-        if (valid < kBN) {  // values past the block's keys: zeros, whatever is there
-          const uint32_t va = smem_addr(ring) + (it % kStages) * 2 * kTile;
-          for (int r = max(valid, 0) + (lane >> 3); r < kBN; r += 4)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(va + h * kHalf + r * 128 + (lane & 7) * 16), "r"(0)
-                           : "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (step >= count[i]) continue;
-          if (step == 0) ok = wait_warp(&sh.o_empty[i], (o_seen[i]++ & 1) ^ 1, err);
-          ok = ok && wait_warp(&sh.p_full[i][0], p_seen[i] & 1, err);
-          if (!ok) break;
-          issue_o(i, step == 0, 0);
-          ok = wait_warp(&sh.p_full[i][1], p_seen[i]++ & 1, err);
-          if (!ok) break;
-          issue_o(i, step == 0, 1);
-          // The next scores overwrite this tile's P: one thread's MMAs run in the order of their issue.
-          if (step + 1 < count[i]) issue_s(i);
-          else commit(&sh.o_full[i]);
-        }
-        if (!ok) break;
+        for (int i = 0; i < 2; ++i)
+          if (count[i] > 0) issue_s(i);
         commit(&sh.pair_empty[it % kStages]);
-        if (step + 2 == steps) commit(&sh.q_empty);
+        if (steps == 1) commit(&sh.q_empty);
+        ++it;
+        for (int step = 0; step < steps; ++step, ++it) {
+          if (!wait_pair()) {
+            ok = false;
+            break;
+          }
+          const int valid = left - step * kBN;
+          if (valid < kBN) {  // values past the block's keys: zeros, whatever is there
+            const uint32_t va = smem_addr(ring) + (it % kStages) * 2 * kTile;
+            for (int r = max(valid, 0) + (lane >> 3); r < kBN; r += 4)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(va + h * kHalf + r * 128 + (lane & 7) * 16), "r"(0)
+                             : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (step >= count[i]) continue;
+            if (step == 0) ok = wait_warp(&sh.o_empty[i], (o_seen[i]++ & 1) ^ 1, err);
+            ok = ok && wait_warp(&sh.p_full[i][0], p_seen[i] & 1, err);
+            if (!ok) break;
+            issue_o(i, step == 0, 0);
+            ok = wait_warp(&sh.p_full[i][1], p_seen[i]++ & 1, err);
+            if (!ok) break;
+            issue_o(i, step == 0, 1);
+            // The next scores overwrite this tile's P: one thread's MMAs run in the order of their issue.
+            if (step + 1 < count[i]) issue_s(i);
+            else commit(&sh.o_full[i]);
+          }
+          if (!ok) break;
+          commit(&sh.pair_empty[it % kStages]);
+          if (step + 2 == steps) commit(&sh.q_empty);
+        }
       }
+      if (!ok) *abort_flag = 1;
     }
-    if (!ok) *abort_flag = 1;
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax, one row per thread
@@ -779,24 +812,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                    : kShared ? a.whole + out_row * kRecord
                              : nullptr;
       const int at_m = part ? kBlockRows * 128 - record_row * 7 : 128, at_sum = part ? at_m + kBlockRows : 129;
-      const bool sees = limit > w.tile0 * kBN;  // a key of this piece; else its weights are none, whatever they met
-      const float inv = rec ? 1.f : 1.f / l;
+      const bool sees = limit > w.tile0 * kBN;  // a key of this piece; else its weights are none
+      const float inv = !sees ? 0.f : rec ? 1.f : 1.f / l;
       float largest = 0.f;  // NaN if something is
       if (count > 0) {
         // Rows go out through shared memory, 64 bytes of 8 rows per store: 16 bytes of 32 rows each would
         // take the L1 a cycle per row and store, 4000 for the two tiles.
-        const int out_rows = real ? static_cast<int>(out_row) : -1;
+        const int mine = real ? static_cast<int>(out_row) : -1;
+        int rows[4];  // whose pieces this lane stores
+#pragma unroll
+        for (int q = 0; q < 4; ++q) rows[q] = __shfl_sync(0xffffffffu, mine, q * 8 + (lane >> 2));
         uint4* stage = sh.stage[warp];
-#pragma unroll 1
+        uint32_t o[2][32];
+        float large[4] = {0.f, 0.f, 0.f, 0.f};
+        tmem_ld32(t_o, o[0]);
+#pragma unroll 2
         for (int b = 0; b < kD / 32; ++b) {
-          uint32_t o[32];
-          tmem_ld32(t_o + b * 32, o);
-          tmem_ld_wait(o);
+          uint32_t* ob = o[b & 1];
+          tmem_ld_wait(ob);
+          tmem_ld32(t_o + (b + 1 < kD / 32 ? b + 1 : 0) * 32, o[(b + 1) & 1]);  // the last one: read again, not used
           float f[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = sees ? __uint_as_float(o[e]) * inv : 0.f;
+          for (int e = 0; e < 16; ++e)
+            unpair(mul2(pair(__uint_as_float(ob[2 * e]), __uint_as_float(ob[2 * e + 1])), pair(inv, inv)), &f[2 * e],
+                   &f[2 * e + 1]);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) largest = max3(largest, fabsf(f[2 * e]), fabsf(f[2 * e + 1]));
+          for (int e = 0; e < 16; ++e) large[e & 3] = max3(large[e & 3], fabsf(f[2 * e]), fabsf(f[2 * e + 1]));
           if (rec) {
             if (real) {
 #pragma unroll
@@ -808,16 +849,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) stage[lane * 4 + (e ^ (lane >> 1 & 3))] = pack8(f + 8 * e);
             __syncwarp();
+            uint4 y[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const int from = q * 8 + (lane >> 2), row = __shfl_sync(0xffffffffu, out_rows, from);
-              if (row >= 0)
-                *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(row) * 128 + b * 32 + (lane & 3) * 8) =
-                    stage[from * 4 + ((lane & 3) ^ (from >> 1 & 3))];
+              const int from = q * 8 + (lane >> 2);
+              y[q] = stage[from * 4 + ((lane & 3) ^ (from >> 1 & 3))];
             }
             __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (rows[q] >= 0)
+                *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(rows[q]) * 128 + b * 32 + (lane & 3) * 8) = y[q];
           }
         }
+        tmem_ld_wait(o[0]);
+        largest = max3(max3(large[0], large[1], large[2]), large[3], large[3]);
         tc_fence_before();
         mbar_arrive(&sh.o_empty[i]);
         ++o_seen;
@@ -829,9 +875,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         rec[at_sum] = sees ? l : 0.f;
       }
       // rows with something not finite: again, key by key
-      unsigned again = __ballot_sync(0xffffffffu, real && sees && count > 0 && (odd || !(largest <= 3.4e38f)));
+      unsigned again = __ballot_sync(0xffffffffu, real && count > 0 && (odd || !(largest <= 3.4e38f)));
       __syncwarp();
-      while (again) {
+      while (__builtin_expect(again != 0, 0)) {
         const int from = __ffs(again) - 1;
         again &= again - 1;
         const int64_t row = __shfl_sync(0xffffffffu, out_row, from);
@@ -846,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             rec[at_sum] = sum;
           }
         } else {
-          const float s = 1.f / sum;
+          const float s = keys > first ? 1.f / sum : 0.f;
           *reinterpret_cast<uint2*>(a.out + row * 128 + lane * 4) =
               make_uint2(pack_bf16x2(o[0] * s, o[1] * s), pack_bf16x2(o[2] * s, o[3] * s));
         }
