@@ -30,8 +30,8 @@ struct PagedCache {
 
   __device__ __forceinline__ int page_size() const { return 1 << page_shift; }
   // a sequence's length, 0 (and device error 2) where it does not fit its row of the page table
-  __device__ __forceinline__ int length(int s) const {
-    const int n = __ldg(lengths + s);
+  __device__ __forceinline__ int length(int s) const { return checked_length(__ldg(lengths + s)); }
+  __device__ __forceinline__ int checked_length(int n) const {
     if (n >= 0 && n <= (static_cast<int64_t>(max_pages) << page_shift)) return n;
     report(err, kErrPositionRange);
     return 0;

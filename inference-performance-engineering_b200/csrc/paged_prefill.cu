@@ -179,6 +179,17 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* e
   return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_longer(bar, parity, err);
 }
 
+// whether a phase is complete, at once
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return yes != 0;
+}
+
 // the largest of three; NaN if one is
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -243,12 +254,12 @@ struct Span {
   int begin, tokens, length;
 };
 __device__ __forceinline__ Span span_of(const PagedCache& c, int s, int rows) {
-  const int b = __ldg(c.cu_tokens + s), e = __ldg(c.cu_tokens + s + 1);
+  const int b = __ldg(c.cu_tokens + s), e = __ldg(c.cu_tokens + s + 1), n = __ldg(c.lengths + s);
   if (b < 0 || e < b || e > rows) {
     report(c.err, kErrPositionRange);
     return Span{0, 0, 0};
   }
-  const int length = c.length(s);
+  const int length = c.checked_length(n);
   if (e - b > length) report(c.err, kErrPositionRange);
   return Span{b, e - b, length};
 }
@@ -362,6 +373,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
       int blocks = 0, tiles = 0, most = 0;
       bool whole = false;
+      Span mine{0, 0, 0};  // of sequence `lane`
+      auto span_at = [&](int s) {  // of any, for a whole warp
+        if (c.sequences > 32) return span_of(c, s, a.tokens);
+        return Span{__shfl_sync(0xffffffffu, mine.begin, s), __shfl_sync(0xffffffffu, mine.tokens, s),
+                    __shfl_sync(0xffffffffu, mine.length, s)};
+      };
       if (kShared) {
         blocks = (a.tokens + per_block - 1) / per_block;
         tiles = blocks * shared_tiles;
@@ -370,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int s = base + lane;
           Span x{0, 0, 0};
           if (s < c.sequences) x = span_of(c, s, a.tokens);
+          if (base == 0) mine = x;
           const int n = (x.tokens + per_block - 1) / per_block, first = max(0, x.length - x.tokens) / per_block;
           const int before = blocks + warp_scan(n);
           if (s < kMaxListed) {
@@ -388,11 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         int longest = 0;
         for (int base = 0; base < blocks; base += 32) {
           const int i = base + lane;
-          int n = 0;
-          if (i < blocks) {
-            const int s = last_at_most(sh.low, c.sequences, i);
-            n = tiles_of(block_keys(span_of(c, s, a.tokens), i - sh.low[s], per_block));
-          }
+          const int s = last_at_most(sh.low, c.sequences, min(i, blocks - 1));
+          const Span x = span_at(s);
+          const int n = i < blocks ? tiles_of(block_keys(x, i - sh.low[s], per_block)) : 0;
           const int before = tiles + warp_scan(n);
           if (i < blocks) sh.high[i] = before;
           longest = max(longest, n);
@@ -488,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 2; ++i) w.count[i] = w.tokens > i * per_tile ? tile1 - tile0 : 0;
           } else {
             const int s = last_at_most(sh.low, c.sequences, block);
-            w = make_work(span_of(c, s, a.tokens), s, block - sh.low[s], kv_head, per_tile, tile0, whole ? -1 : tile1);
+            w = make_work(span_at(s), s, block - sh.low[s], kv_head, per_tile, tile0, whole ? -1 : tile1);
             if (tile0 == 0 && kv_head == 0 && lane == 0) a.blocks[block] = make_int4(w.token0, w.tokens, w.position0, 0);
           }
           if (tile0 > 0 || tile1 < n) w.record = static_cast<int>(blockIdx.x) * 2 + (round == 0 ? 0 : 1);
@@ -504,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } while (rank >= works);
           int s, b;
           select(rank / c.kv_heads, &s, &b);
-          w = make_work(span_of(c, s, a.tokens), s, b, rank % c.kv_heads, per_tile, 0, -1);
+          w = make_work(span_at(s), s, b, rank % c.kv_heads, per_tile, 0, -1);
         }
         *out = w;
         return true;
@@ -540,6 +556,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           has = has_page(w, 0);
           has_v = false;
         }
+        // The block's queries, once the piece before is done with its own: at once if it is, else after the keys.
+        auto send_queries = [&] {
+          if (lane == 0) {
+            sh.work[piece & 1] = w;
+            const int rows = group * per_tile * 128;  // bytes of a query tile's half
+            const int n = w.tokens > per_tile ? 2 : 1;
+            mbar_expect_tx(&sh.q_full, 2 * rows * n);
+            for (int i = 0; i < n; ++i) {
+              const uint32_t dst_q = smem_addr(s_q) + i * kTile;
+              tma_load_3d(dst_q, &map_q, &sh.q_full, 0, w.kv_head * group, w.token0 + i * per_tile);
+              tma_load_3d(dst_q + kHalf, &map_q, &sh.q_full, 64, w.kv_head * group, w.token0 + i * per_tile);
+            }
+          }
+          __syncwarp();
+          ++piece;
+        };
+        const bool early = step == 0 && __all_sync(0xffffffffu, mbar_test(&sh.q_empty, (piece & 1) ^ 1));
+        if (early) send_queries();
         // keys of `step`, values of the step before
         if (has) row = static_cast<int>(c.page_row(c.checked(id), w.kv_head));
         id = load_id(w, step + 1);
@@ -560,24 +594,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_2d(dst + kTile + kHalf, &map_k, &sh.pair_full[slot], 64, row);
         }
         armed = (armed & ~(1u << slot)) | (phase << slot) | (1u << (16 + slot));
-        if (step == 0) {  // the block's queries, once the piece before is done with its own
+        if (step == 0 && !early) {
           if (!wait_warp(&sh.q_empty, (piece & 1) ^ 1, err)) {
             ok = false;
             break;
           }
-          if (lane == 0) {
-            sh.work[piece & 1] = w;
-            const int rows = group * per_tile * 128;  // bytes of a query tile's half
-            const int n = w.tokens > per_tile ? 2 : 1;
-            mbar_expect_tx(&sh.q_full, 2 * rows * n);
-            for (int i = 0; i < n; ++i) {
-              const uint32_t dst_q = smem_addr(s_q) + i * kTile;
-              tma_load_3d(dst_q, &map_q, &sh.q_full, 0, w.kv_head * group, w.token0 + i * per_tile);
-              tma_load_3d(dst_q + kHalf, &map_q, &sh.q_full, 64, w.kv_head * group, w.token0 + i * per_tile);
-            }
-          }
-          __syncwarp();
-          ++piece;
+          send_queries();
         }
         if (++slot == kStages) {
           slot = 0;
@@ -596,6 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         *abort_flag = 1;
+        if (piece > 0) mbar_wait(&sh.q_full, (piece - 1) & 1, err);
       }
       // copies and arrivals in flight land before the CTA's shared memory goes away
       for (int s = 0; s < kStages; ++s) {
