@@ -849,11 +849,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t o[2][32];
         float large[4] = {0.f, 0.f, 0.f, 0.f};
         tmem_ld32(t_o, o[0]);
+        tmem_ld_wait(o[0]);
 #pragma unroll 2
         for (int b = 0; b < kD / 32; ++b) {
           uint32_t* ob = o[b & 1];
-          tmem_ld_wait(ob);
-          tmem_ld32(t_o + (b + 1 < kD / 32 ? b + 1 : 0) * 32, o[(b + 1) & 1]);  // the last one: read again, not used
+          uint32_t* next = o[(b + 1) & 1];
+          tmem_ld32(t_o + (b + 1 < kD / 32 ? b + 1 : 0) * 32, next);  // the last one: read again, not used
           float f[32];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -884,8 +885,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (rows[q] >= 0)
                 *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(rows[q]) * 128 + b * 32 + (lane & 3) * 8) = y[q];
           }
+          tmem_ld_wait(next);  // here, so that no register of a load in flight is moved or read
         }
-        tmem_ld_wait(o[0]);
         largest = max3(max3(large[0], large[1], large[2]), large[3], large[3]);
         tc_fence_before();
         mbar_arrive(&sh.o_empty[i]);
@@ -933,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // The blocks whose key tiles lie in more than one run: a CTA per (block, KV head, 8 rows), a warp per row.
-constexpr int kMergeRows = 8;
+constexpr int kMergeRows = 4;
 __global__ void __launch_bounds__(kMergeRows * 32) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
   const int block = blockIdx.x / a.c.kv_heads, kv_head = blockIdx.x - block * a.c.kv_heads;
   const int group = a.q_heads / a.c.kv_heads, per_tile = kBM / group;
