@@ -248,7 +248,10 @@ int ipe_prefill_attention(const void* q, const void* k_cache, const void* v_cach
  * The integers are read on the device only, so a captured call replays with other values. A length that is
  * negative, larger than max_pages * page_size or less than the sequence's new tokens sets device error 2, a page
  * outside [0, num_pages) device error 5; such a sequence's output rows hold no meaning, the others are served and
- * nothing outside the buffers is touched. Outputs must not overlap inputs. */
+ * nothing outside the buffers is touched. Outputs must not overlap inputs. A page may stand in several rows of the
+ * table, but not where two of them append: sequences that share a page only read it. Workspaces are 256-byte
+ * aligned, as large as the _workspace function says on the device of the call, of any contents, and belong to the
+ * call until it has run. */
 
 /* ipe_qk_norm_rope_append (src/ipe/forward.py:101-109) for a ragged batch and a paged cache: token i of the n
  * that a sequence brings is at position lengths[s] - n + i. Computed in fp32 and rounded to bf16 once.
@@ -264,8 +267,7 @@ int ipe_paged_qk_norm_rope_append(const void* qkv, int64_t tokens, int q_heads, 
                                   int64_t num_pages, int page_size, float eps, void* stream);
 
 /* One query token per sequence, q bf16 [sequences, q_heads, 128], over keys 0 .. lengths[s] - 1: out bf16
- * [sequences, q_heads * 128] (src/ipe/ops.py:78-101, decode). Length 0 gives zeros. The workspace is 256-byte
- * aligned, of any contents, and belongs to the call until it has run. */
+ * [sequences, q_heads * 128] (src/ipe/ops.py:78-101, decode). Length 0 gives zeros. */
 int ipe_paged_decode_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                const int32_t* lengths, void* out, int sequences, int q_heads, int kv_heads,
                                int64_t num_pages, int page_size, int max_pages, void* workspace,

@@ -40,7 +40,7 @@ int paged_cache(const char* name, const void* k_pages, const void* v_pages, cons
                 static_cast<long long>(tokens), sequences, static_cast<long long>(num_pages), max_pages);
   // positions, cache rows, (token, head) rows and units of 64 keys are 32-bit numbers in the kernels; their
   // byte offsets are 64-bit
-  if (tokens * q_heads > INT32_MAX || num_pages > INT32_MAX / (static_cast<int64_t>(kv_heads) * page_size) ||
+  if (tokens > INT32_MAX / q_heads || num_pages > INT32_MAX / (static_cast<int64_t>(kv_heads) * page_size) ||
       max_pages > (1 << 27) / page_size || sequences > (1 << 24) ||
       static_cast<int64_t>(sequences) * kv_heads > INT32_MAX / (static_cast<int64_t>(max_pages) * page_size / 64 + 1))
     return fail(IPE_ERR_UNSUPPORTED, "%s: sizes past the kernels' 32-bit row numbers", name);

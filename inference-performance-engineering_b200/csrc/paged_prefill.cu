@@ -1,8 +1,8 @@
 // Causal attention of ragged new tokens over a paged cache, on the 5th-generation tensor cores.
 //
 // A block of work is up to 256 query rows of one (sequence, KV head): two tiles of 128 rows, a row being
-// one of the G query heads of one token (tokens of 128 / G, whole), so the G heads share every key that
-// is read. Per key tile of 128 keys and query tile: S = Q K^T (tcgen05.mma into tensor memory), a row
+// one of the G query heads of one token (128 / G whole tokens to a tile), so the G heads share every key
+// that is read. Per key tile of 128 keys and query tile: S = Q K^T (tcgen05.mma into tensor memory), a row
 // per thread reads its scores, keeps an fp32 running maximum and sum in base 2, writes P over the scores
 // as bf16, and O += P V takes P from tensor memory. The two query tiles take turns: while one's scores
 // are in the softmax warps the tensor cores work on the other's products.
@@ -12,11 +12,19 @@
 // scores pass it by 2^8 (weights up to 256 are as exact in bf16 and fp32 as weights up to 1), so the
 // accumulator in tensor memory is rescaled a few times per row instead of at every tile.
 //
+// Bound, on long prompts, by the chain of a tile: a step (128 keys of both query tiles) is 2070 cycles of
+// products and takes about 2950, with the scores' way through the softmax warps (1400 cycles per tile, the
+// special function unit half busy) and back between two products of the same tile. 8192 new tokens, 16 query
+// heads over 8: 219 us, 1250 TFLOP/s of the products below the diagonal (0.76 of the measured peak). A
+// sixteenth of that work, nine prompts of 17 to 2500 tokens, 32 heads over 8: 119 us, 950 TFLOP/s; there the
+// change from one piece to the next counts (3 us before the next piece was looked up ahead). Pieces of two
+// prompts on 9000 to 20000 cached tokens: 60 us, 2 TB/s. 512 tokens: 20 us, a chain of launches and lookups.
+//
 // Warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread; warp 8: work list and TMA loads;
 // warp 9: tensor memory and MMA issue. Persistent, one CTA per SM; the blocks go to the CTAs heaviest
-// first, back and forth. Where there are fewer blocks than that can balance, every block's key tiles are
-// dealt to the CTAs in equal contiguous runs instead; parts of a block go to the workspace as records (unnormalised o, maximum, sum),
-// merged by a second kernel in order of the keys.
+// first, back and forth. Where there are fewer blocks than that can balance (two per SM), every block's key
+// tiles are dealt to the CTAs in equal contiguous runs instead; parts of a block go to the workspace as
+// records (unnormalised o, maximum, sum), merged by a second kernel in order of the keys.
 //
 // Values past a block's last key are zeroed in shared memory before they meet their zero weights. A row
 // whose accumulator is not finite all the same (a value that is infinite or NaN, its own or one of a

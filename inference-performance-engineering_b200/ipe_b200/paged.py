@@ -116,7 +116,7 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: t
 
     qkv [rows, (Hq + 2 Hkv) * 128] (q | k | v per token), q_norm / k_norm [128], cos / sin [positions, 128]
     bf16 or fp32, q_out [rows, Hq, 128]. Computed in fp32 and rounded to bf16 once. A position past the tables
-    sets device error 2, and its row is skipped.
+    sets device error 2, and its row is skipped. Sequences may share pages that they read, not one that they append to.
     """
     name = "paged_qk_norm_rope_append"
     device = _device(name, k_pages)
