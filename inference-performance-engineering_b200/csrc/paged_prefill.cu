@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       // the `rank`-th block in descending order of its number; the whole warp takes part
-      int low0, high0;
-      range_of(lane, &low0, &high0);
+      int low0 = 0, high0 = 0;  // of sequence `lane`
+      if (!in_runs) range_of(lane, &low0, &high0);
       auto select = [&](int rank, int* seq, int* block) {
         auto at_least = [&](int x) {
           int n = max(0, high0 - max(low0, x));

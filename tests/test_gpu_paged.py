@@ -366,6 +366,13 @@ def test_shared_prefix(lengths, prefix, page, q_heads, kv_heads):
     assert (out[b.lengths == 0] == 0).all()
 
 
+@pytest.mark.parametrize(("q_heads", "kv_heads"), [(4, 2), (3, 1)])
+def test_shared_prefix_of_more_sequences_than_are_listed(q_heads, kv_heads):
+    b = Batch([1] * 1100, [n % 90 for n in range(1100)], 32, kv_heads, seed=29, prefix=2).fill(970)
+    q = normal((1100, q_heads, 128), 30, 1.5)
+    check(shared(b, q), b, q)
+
+
 @pytest.mark.parametrize("bad", [NAN, float("inf"), torch.finfo(torch.bfloat16).min])
 def test_shared_keys_behind_a_rows_end(bad):
     """A sequence that ends inside the prefix sees nothing of the prefix's later keys, whatever they hold."""
