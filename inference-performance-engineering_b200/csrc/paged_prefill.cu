@@ -961,7 +961,7 @@ __global__ void __launch_bounds__(kMergeRows * 32) paged_prefill_merge_kernel(co
   if (b.z + token < 0)  // no position: no keys
     *reinterpret_cast<uint2*>(row + (threadIdx.x & 31) * 4) = make_uint2(0u, 0u);
   else
-    join_parts(parts, row);
+    join_parts<8>(parts, row);
 }
 
 // most blocks that `tokens` new tokens of `sequences` sequences make

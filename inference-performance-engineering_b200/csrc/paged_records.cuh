@@ -74,8 +74,7 @@ struct Parts {
 
 // Joins the parts in order, by a whole warp; lane l writes elements 4l..4l+3 of the bf16 row `out`. Up to
 // kTogether records are loaded at once; a later group's maximum rescales what the groups before gave.
-constexpr int kTogether = 8;
-template <int N>
+template <int kTogether, int N>
 __device__ __forceinline__ void join_parts(const Parts (&parts)[N], bf16* out) {
   float top = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
