@@ -688,9 +688,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 2; ++i)
-          if (count[i] > 0) issue_s(i);
+          if ((i ? count[1] : count[0]) > 0) issue_s(i);
         commit(&sh.pair_empty[it % kStages]);
         if (steps == 1) commit(&sh.q_empty);
         ++it;
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (step > 0 && __any_sync(0xffffffffu, moves)) {  // the products of the tile before have finished: S came after
           const float keep = exp2_approx(m * kScaleLog2 - base);
           l *= moves ? keep : 1.f;
-#pragma unroll
+#pragma unroll 1
           for (int b = 0; b < kD / 32; ++b) {
             uint32_t o[32];
             tmem_ld32(t_o + b * 32, o);
@@ -854,15 +854,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) rows[q] = __shfl_sync(0xffffffffu, mine, q * 8 + (lane >> 2));
         uint4* stage = sh.stage[warp];
-        uint32_t o[2][32];
         float large[4] = {0.f, 0.f, 0.f, 0.f};
-        tmem_ld32(t_o, o[0]);
-        tmem_ld_wait(o[0]);
-#pragma unroll 2
+#pragma unroll 1
         for (int b = 0; b < kD / 32; ++b) {
-          uint32_t* ob = o[b & 1];
-          uint32_t* next = o[(b + 1) & 1];
-          tmem_ld32(t_o + (b + 1 < kD / 32 ? b + 1 : 0) * 32, next);  // the last one: read again, not used
+          uint32_t ob[32];
+          tmem_ld32(t_o + b * 32, ob);
+          tmem_ld_wait(ob);
           float f[32];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
@@ -893,7 +890,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (rows[q] >= 0)
                 *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(rows[q]) * 128 + b * 32 + (lane & 3) * 8) = y[q];
           }
-          tmem_ld_wait(next);  // here, so that no register of a load in flight is moved or read
         }
         largest = max3(max3(large[0], large[1], large[2]), large[3], large[3]);
         tc_fence_before();
