@@ -15,10 +15,11 @@
 // Bound, on long prompts, by the chain of a tile: a step (128 keys of both query tiles) is 2070 cycles of
 // products and takes about 2950, with the scores' way through the softmax warps (1400 cycles per tile, the
 // special function unit half busy) and back between two products of the same tile. 8192 new tokens, 16 query
-// heads over 8: 219 us, 1250 TFLOP/s of the products below the diagonal (0.76 of the measured peak). A
-// sixteenth of that work, nine prompts of 17 to 2500 tokens, 32 heads over 8: 119 us, 950 TFLOP/s; there the
-// change from one piece to the next counts (3 us before the next piece was looked up ahead). Pieces of two
-// prompts on 9000 to 20000 cached tokens: 60 us, 2 TB/s. 512 tokens: 20 us, a chain of launches and lookups.
+// heads over 8: 217 us, 1260 TFLOP/s of the products below the diagonal (0.77 of the measured peak). Nine
+// prompts of 17 to 2500 tokens, 32 heads over 8: 115 us, 980 TFLOP/s; there the change from one piece to the
+// next counts, 6000 cycles beside a step's. Much of them is instruction fetch, so what runs once per piece stands
+// in rolled loops (119 us with them unrolled). Pieces of two prompts on 9000 to 20000 cached tokens: 57 to 68
+// us, about 2 TB/s. 512 tokens: 20 us, a chain of launches and lookups.
 //
 // Warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread; warp 8: work list and TMA loads;
 // warp 9: tensor memory and MMA issue. Persistent, one CTA per SM; the blocks go to the CTAs heaviest
