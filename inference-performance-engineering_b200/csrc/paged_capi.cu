@@ -88,7 +88,7 @@ size_t ipe_paged_prefill_attention_workspace(int64_t tokens, int sequences, int 
 }
 
 size_t ipe_shared_prefix_attention_workspace(int sequences, int q_heads, int kv_heads, int page_size, int prefix_count) {
-  if (sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8 || page_size < 1 || prefix_count < 0)
+  if (sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8 || page_size < 1 || page_size > 128 || prefix_count < 0)
     return 0;
   ipe::PagedCache c{};
   c.sequences = sequences;

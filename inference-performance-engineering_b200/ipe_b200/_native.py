@@ -9,8 +9,10 @@ their arguments on the host before launching anything.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from ctypes import c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
+from types import ModuleType
 
 LIBRARY = Path(__file__).resolve().parent / "lib" / "libipe_b200.so"
 
@@ -141,6 +143,25 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+_calls: ModuleType | None = None
+
+
+def paged_calls() -> ModuleType:
+    """The extension module that launches the paged operators' ordinary calls (csrc/paged_calls.cpp)."""
+    global _calls
+    if _calls is None:
+        load()
+        path = LIBRARY.with_name("_paged_calls.so")
+        spec = importlib.util.spec_from_file_location("_paged_calls", path)
+        try:
+            module = importlib.util.module_from_spec(spec)
+        except ImportError as error:
+            raise NativeUnavailable(f"cannot load {path}: build it with `python -m ipe_b200.build` ({error})") from error
+        spec.loader.exec_module(module)
+        _calls = module
+    return _calls
 
 
 def check(status: int, name: str) -> None:

@@ -4,7 +4,8 @@
 
 Each `csrc/*.cu` compiles to an object for `-gencode arch=compute_100a,code=sm_100a` (the only
 target: tcgen05 and TMA need the `a` variant), then one `-shared` link with the CUDA runtime linked
-statically. Nothing else is built; no JIT cache is used.
+statically. `csrc/paged_calls.cpp`, the Python functions of the paged operators, becomes the extension
+module `ipe_b200/lib/_paged_calls.so` beside it, against the torch that runs this. No JIT cache is used.
 """
 
 from __future__ import annotations
@@ -13,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -22,6 +24,7 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB_DIR = PACKAGE / "lib"
 LIBRARY = LIB_DIR / "libipe_b200.so"
+CALLS = LIB_DIR / "_paged_calls.so"
 BUILD_DIR = ROOT / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -73,7 +76,29 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
         result = subprocess.run(cmd, capture_output=True, text=True)
         if result.returncode != 0:
             raise RuntimeError(f"link failed:\n{result.stderr}")
+    build_calls(verbose)
     return LIBRARY
+
+
+def build_calls(verbose: bool = False) -> Path:
+    source = CSRC / "paged_calls.cpp"
+    if not _stale(CALLS, [source, *INCLUDE.glob("*.h")]):
+        return CALLS
+    import torch
+
+    torch_root = Path(torch.__file__).resolve().parent
+    includes = [torch_root / "include", torch_root / "include" / "torch" / "csrc" / "api" / "include",
+                Path(nvcc()).resolve().parent.parent / "include", sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", *(f"-isystem{path}" for path in includes),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(source), "-o", str(CALLS),
+           f"-L{torch_root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{LIB_DIR}", "-lipe_b200",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"g++ failed on {source.name}:\n{result.stderr}")
+    return CALLS
 
 
 if __name__ == "__main__":

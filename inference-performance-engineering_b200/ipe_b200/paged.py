@@ -31,9 +31,11 @@ import torch
 
 from ipe_b200 import _native as nat
 
-# The checks run on every call of a step whose kernels take a few microseconds, so what follows from the
-# tensors' shapes alone (their agreement, the sizes the kernels get, the workspace) is worked out once per
-# set of shapes.
+# An ordinary call is checked and launched by csrc/paged_calls.cpp: the kernels of a small step take a few
+# microseconds, the same work here takes the host 10 to 13. A call that it does not take (None) comes here, where the
+# checks say what is wrong with it; what passes them, a call on another device than the current one or of
+# subclasses of Tensor, is launched from here. What follows from the tensors' shapes alone (their agreement, the
+# sizes the kernels get, the workspace) is worked out once per set of shapes.
 
 
 def _check(name: str, dtype: torch.dtype, labels: tuple[str, ...], tensors: tuple[torch.Tensor, ...], device: int) -> None:
@@ -102,6 +104,13 @@ def _attention_sizes(name, device, q, k_pages, v_pages, page_table, lengths, out
     return (*sizes, q[1], int(workspace))
 
 
+def _launched(status: int | None, name: str) -> bool:
+    """Whether the extension module took the call; an entry point's refusal is raised."""
+    if status:
+        nat.check(status, "ipe_" + name)
+    return status is not None
+
+
 def _elsewhere(device, function, *args):
     """The call under its tensors' device, to which its launches, workspace and stream belong."""
     with torch.cuda.device(device):
@@ -119,6 +128,9 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: t
     sets device error 2, and its row is skipped. Sequences may share pages that they read, not one that they append to.
     """
     name = "paged_qk_norm_rope_append"
+    if _launched(nat.paged_calls().paged_qk_norm_rope_append(qkv, q_norm, k_norm, cos, sin, cu_tokens, lengths, page_table, eps, q_out, k_pages,
+            v_pages), name):
+        return q_out
     device = _device(name, k_pages)
     if device != torch._C._cuda_getDevice():
         return _elsewhere(device, paged_qk_norm_rope_append, qkv, q_norm, k_norm, cos, sin, cu_tokens, lengths, page_table, eps,
@@ -146,6 +158,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """out [S, Hq * 128] = softmax(q k^T / sqrt(128)) v over keys 0 .. lengths[s] - 1 of every sequence, one query
     token q [S, Hq, 128] each, 1 to 8 query heads per KV head. A sequence of length 0 gives zeros."""
     name = "paged_decode_attention"
+    if _launched(nat.paged_calls().paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out), name):
+        return out
     device = _device(name, k_pages)
     if device != torch._C._cuda_getDevice():
         return _elsewhere(device, paged_decode_attention, q, k_pages, v_pages, page_table, lengths, out)
@@ -167,6 +181,8 @@ def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     """Causal attention of ragged new tokens q [rows, Hq, 128] over their sequences' pages: token i of the n that
     sequence s brings sees keys 0 .. lengths[s] - n + i. out [rows, Hq * 128]; 1 to 8 query heads per KV head."""
     name = "paged_prefill_attention"
+    if _launched(nat.paged_calls().paged_prefill_attention(q, k_pages, v_pages, page_table, cu_tokens, lengths, out), name):
+        return out
     device = _device(name, k_pages)
     if device != torch._C._cuda_getDevice():
         return _elsewhere(device, paged_prefill_attention, q, k_pages, v_pages, page_table, cu_tokens, lengths, out)
@@ -191,6 +207,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     sequence] is read for the positions behind it alone (its first prefix_pages.numel() columns may hold anything).
     lengths [S] count the prefix; a sequence that ends inside the prefix sees its own lengths[s] keys of it."""
     name = "shared_prefix_attention"
+    if _launched(nat.paged_calls().shared_prefix_attention(q, k_pages, v_pages, prefix_pages, page_table, lengths, out), name):
+        return out
     device = _device(name, k_pages)
     if device != torch._C._cuda_getDevice():
         return _elsewhere(device, shared_prefix_attention, q, k_pages, v_pages, prefix_pages, page_table, lengths, out)

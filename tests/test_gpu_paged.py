@@ -580,6 +580,32 @@ def test_the_registered_operators():
     assert torch.equal(b.v[pages, :, rows][0], qkv[0].view(8, 128)[6:])
 
 
+def test_subclasses_of_tensor_and_whole_numbers():
+    """What the extension module leaves to the Python checks gives the same bits."""
+    class Other(torch.Tensor):
+        pass
+
+    b = Batch([3, 1], [40, 50], 16, 2, seed=97, prefix=1).fill(1500)
+    qkv, w = normal((4, 8 * 128), 98), torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    cos, sin = normal((60, 128), 99, dtype=torch.float32), normal((60, 128), 100, dtype=torch.float32)
+    b.page_table[:, :1] = b.prefix_pages
+    rows = []
+    for eps, change in ((1.0, lambda t: t), (1, lambda t: t), (1.0, lambda t: t.as_subclass(Other)),
+                        (1.0, lambda t: torch.nn.Parameter(t, requires_grad=False))):
+        q = torch.empty(4, 4, 128, dtype=torch.bfloat16, device=DEV)
+        k, v, table, lengths = change(b.k.clone()), change(b.v.clone()), change(b.page_table), change(b.lengths)
+        ops.paged_qk_norm_rope_append(change(qkv), w, w, cos, sin, b.cu, lengths, table, eps, change(q), k, v)
+        outs = [torch.empty(4, 512, dtype=torch.bfloat16, device=DEV) for _ in range(3)]
+        ops.paged_prefill_attention(change(q), k, v, table, b.cu, lengths, outs[0])
+        ops.paged_decode_attention(q[2:].contiguous(), k, v, table, lengths, change(outs[1][:2]))
+        ops.shared_prefix_attention(change(q[2:].contiguous()), k, v, b.prefix_pages, table, lengths, outs[2][:2])
+        rows.append([q, k, v, outs[0], outs[1][:2], outs[2][:2]])
+    for other in rows[1:]:
+        for x, y in zip(rows[0], other):
+            assert torch.equal(torch.nan_to_num(x.as_subclass(torch.Tensor).detach()), torch.nan_to_num(y.as_subclass(torch.Tensor).detach()))
+    assert nat.device_error() == 0
+
+
 def test_refusals_of_the_python_functions():
     b = Batch([1] * 2, [40, 50], 16, 2, seed=95)
     q = normal((2, 4, 128), 96)

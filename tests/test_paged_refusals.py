@@ -89,6 +89,23 @@ def test_the_workspaces_sizes():
     assert lib.ipe_shared_prefix_attention_workspace(4, 16, 8, 16, 9) > lib.ipe_paged_decode_attention_workspace(4, 16, 8)
 
 
+def test_no_workspace_for_pages_of_no_size():
+    for page_size in (0, 129, 2 ** 31 - 1):
+        assert nat.load().ipe_shared_prefix_attention_workspace(4, 16, 8, page_size, 9) == 0
+
+
+def test_the_extension_module_leaves_other_calls_to_the_checks():
+    x = torch.zeros(2, 2)
+    calls = nat.paged_calls()
+    for name, n in (("paged_qk_norm_rope_append", 12), ("paged_decode_attention", 6), ("paged_prefill_attention", 7),
+                    ("shared_prefix_attention", 7)):
+        assert getattr(calls, name)(*[x] * n) is None
+        assert getattr(calls, name)(*[None] * n) is None
+        assert getattr(calls, name)(*["pages"] * n) is None
+        with pytest.raises(TypeError, match=str(n)):
+            getattr(calls, name)(*[x] * (n - 1))
+
+
 def test_cpu_tensors_are_refused():
     pages, table, one = torch.zeros(3, 2, 16, 128, dtype=torch.bfloat16), torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     q, out, cu = torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.zeros(1, 512, dtype=torch.bfloat16), torch.tensor([0, 1], dtype=torch.int32)
