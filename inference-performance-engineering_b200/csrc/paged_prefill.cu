@@ -19,7 +19,7 @@
 // prompts of 17 to 2500 tokens, 32 heads over 8: 115 us, 980 TFLOP/s; there the change from one piece to the
 // next counts, 6000 cycles beside a step's. Much of them is instruction fetch, so what runs once per piece stands
 // in rolled loops (119 us with them unrolled). Pieces of two prompts on 9000 to 20000 cached tokens: 57 to 68
-// us, about 2 TB/s. 512 tokens: 20 us, a chain of launches and lookups.
+// us, about 2 TB/s. 512 tokens: 15 us, a chain of lookups and four steps.
 //
 // Warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread; warp 8: work list and TMA loads;
 // warp 9: tensor memory and MMA issue. Persistent, one CTA per SM; the blocks go to the CTAs heaviest
@@ -263,8 +263,7 @@ __device__ __forceinline__ void attend_row(const PagedCache& c, const bf16* q_ro
 struct Span {
   int begin, tokens, length;
 };
-__device__ __forceinline__ Span span_of(const PagedCache& c, int s, int rows) {
-  const int b = __ldg(c.cu_tokens + s), e = __ldg(c.cu_tokens + s + 1), n = __ldg(c.lengths + s);
+__device__ __forceinline__ Span span_from(const PagedCache& c, int rows, int b, int e, int n) {
   if (b < 0 || e < b || e > rows) {
     report(c.err, kErrPositionRange);
     return Span{0, 0, 0};
@@ -272,6 +271,9 @@ __device__ __forceinline__ Span span_of(const PagedCache& c, int s, int rows) {
   const int length = c.checked_length(n);
   if (e - b > length) report(c.err, kErrPositionRange);
   return Span{b, e - b, length};
+}
+__device__ __forceinline__ Span span_of(const PagedCache& c, int s, int rows) {
+  return span_from(c, rows, __ldg(c.cu_tokens + s), __ldg(c.cu_tokens + s + 1), __ldg(c.lengths + s));
 }
 
 // The piece of block `b` of sequence `s`: key tiles [tile0, tile1) (tile1 < 0: all of them).
@@ -365,6 +367,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
 
+  int first[3] = {0, 0, 0};  // what the list of work begins with, on its way while the CTA is set up
+  if (!kShared && warp == kLoadWarp && lane < c.sequences) {
+    first[0] = __ldg(c.cu_tokens + lane);
+    first[1] = __ldg(c.cu_tokens + lane + 1);
+    first[2] = __ldg(c.lengths + lane);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -397,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int base = 0; base < c.sequences; base += 32) {
           const int s = base + lane;
           Span x{0, 0, 0};
-          if (s < c.sequences) x = span_of(c, s, a.tokens);
-          const int n = (x.tokens + per_block - 1) / per_block, first = max(0, x.length - x.tokens) / per_block;
+          if (s < c.sequences) x = base == 0 ? span_from(c, a.tokens, first[0], first[1], first[2]) : span_of(c, s, a.tokens);
+          const int n = (x.tokens + per_block - 1) / per_block, low = max(0, x.length - x.tokens) / per_block;
           const int before = blocks + warp_scan(n);
           if (base == 0) {
             mine = x;
@@ -406,10 +414,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mine_n = n;
           }
           if (s < kMaxListed) {
-            sh.low[s] = in_runs ? min(before, a.most_blocks) : first;
-            sh.high[s] = first + n;
+            sh.low[s] = in_runs ? min(before, a.most_blocks) : low;
+            sh.high[s] = low + n;
           }
-          if (n > 0) most = max(most, first + n);
+          if (n > 0) most = max(most, low + n);
           blocks = __shfl_sync(0xffffffffu, before + n, 31);
         }
         most = __reduce_max_sync(0xffffffffu, most);
@@ -979,7 +987,7 @@ int64_t most_blocks(int64_t tokens, int sequences, int group) {
 
 // Whether the key tiles are dealt in runs: where whole blocks may leave SMs idle for long, as far as the sizes say.
 // (The kernel looks at the lengths too. A call that it would not cut up in any case needs no merge: 512 tokens on a
-// table of no more 20.0 -> 15.8 us.)
+// table of no more 20.0 and 15.8 us.)
 bool deal_in_runs(int64_t tokens, int sequences, int q_heads, int kv_heads, int64_t most_tiles) {
   const int64_t blocks = most_blocks(tokens, sequences, q_heads / kv_heads), sms = sm_count();
   return blocks <= kMaxListed && sequences <= kMaxListed && blocks * kv_heads < 2 * sms &&
