@@ -118,13 +118,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       const int r = u0 - before * c.kv_heads;
       start = Cursor{s, r / n, r % n, n, keys};
     }
-    if (n == 0 && !a.whole && s % gridDim.x == blockIdx.x) {  // no keys: zeros
-      uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(s) * a.q_heads * 128);
-      for (int i = 0; i < a.q_heads * 16; ++i) row[i] = make_uint4(0, 0, 0, 0);
-    }
-    if (n == 0 && s % gridDim.x == blockIdx.x)
-      for (int h = 0; h < c.kv_heads; ++h) a.items[static_cast<int64_t>(s) * c.kv_heads + h] = make_int2(kNothing, 0);
     before += n;
+  }
+  for (int s = blockIdx.x; s < c.sequences; s += gridDim.x) {  // no keys: zeros
+    if (keys_of(a, s) > 0) continue;
+    for (int h = threadIdx.x; h < c.kv_heads; h += kThreads) a.items[static_cast<int64_t>(s) * c.kv_heads + h] = make_int2(kNothing, 0);
+    if (a.whole) continue;
+    uint4* row = reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(s) * a.q_heads * 128);
+    for (int i = threadIdx.x; i < a.q_heads * 16; i += kThreads) row[i] = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
   if (static_cast<int>(blockIdx.x) >= deal.runs) {
