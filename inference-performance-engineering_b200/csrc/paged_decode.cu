@@ -9,8 +9,10 @@
 // In a unit each of the 4 warps has 16 keys and a running softmax of its own; the warps meet once per
 // piece. S = K q^T and O^T = V^T P^T as m16n8k16 products with the keys (then the head's dimensions) as
 // the 16 rows and the query heads as the 8 columns, so a thread's scores and its output accumulators
-// belong to the same two heads. P enters as two bf16 terms (value and remainder), so the weights keep
-// 16 bits: the products are idle anyway. What a warp waits for (its loads, the chain from scores to weights)
+// belong to the same two heads. P enters as two bf16 terms (the value cut off and the remainder), so the
+// weights keep 16 bits: the products are idle anyway. Neither term of a key with a finite score is ever
+// 0 or negative, nor a factor that rescales what came before 0 (kTiny is the least of them): an infinite
+// value that a row sees stays infinite, with its sign, however small its weight. What a warp waits for (its loads, the chain from scores to weights)
 // the other warps of the SM fill: 3 CTAs with 2 units in flight each against 2 with 3 measured 101.5 and
 // 110.8 us for 160 rows behind a shared prefix, 111.0 and 114.8 for 64 rows of 700 to 12289 keys (6.1 TB/s).
 // 16 rows of 90 to 30001 keys: 57.7 us, 5.2 TB/s, of which the start and the merge take 8; one row of 640
@@ -56,6 +58,20 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+
+// 2^(score - base): 0 for a score of -infinity, else at least kTiny; NaN if the score is
+__device__ __forceinline__ float key_weight(float score, float base) {
+  float p;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(p) : "f"(exp2_approx(score * kScaleLog2 - base)), "f"(kTiny));
+  return score == -INFINITY ? 0.f : p;
+}
+// weights cut off to bf16, and what that leaves of one, above 0 where the weight is
+__device__ __forceinline__ uint32_t cut_bf16x2(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+__device__ __forceinline__ float remainder_of(float p) {
+  return p > 0.f ? fmaxf(p - __uint_as_float(__float_as_uint(p) & 0xffff0000u), kTiny) : 0.f;
 }
 
 // a sequence's keys behind the shared ones
@@ -221,15 +237,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
       for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       top = fmaxf(top, m[e]);
       const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
-      keep[e] = exp2_approx(m[e] * kScaleLog2 - base);
+      keep[e] = part_weight(m[e], base);
       m[e] = top;
-      p[e] = exp2_approx(s4[e] * kScaleLog2 - base);
-      p[2 + e] = exp2_approx(s4[2 + e] * kScaleLog2 - base);
+      p[e] = key_weight(s4[e], base);
+      p[2 + e] = key_weight(s4[2 + e], base);
       l[e] = l[e] * keep[e] + p[e] + p[2 + e];
     }
-    const uint32_t b0 = transpose8x8(pack_bf16x2(p[0], p[1])), b1 = transpose8x8(pack_bf16x2(p[2], p[3]));
-    const uint32_t r0 = transpose8x8(pack_bf16x2(p[0] - bf16_round(p[0]), p[1] - bf16_round(p[1])));
-    const uint32_t r1 = transpose8x8(pack_bf16x2(p[2] - bf16_round(p[2]), p[3] - bf16_round(p[3])));
+    const uint32_t b0 = transpose8x8(cut_bf16x2(p[0], p[1])), b1 = transpose8x8(cut_bf16x2(p[2], p[3]));
+    const uint32_t r0 = transpose8x8(pack_bf16x2(remainder_of(p[0]), remainder_of(p[1])));
+    const uint32_t r1 = transpose8x8(pack_bf16x2(remainder_of(p[2]), remainder_of(p[3])));
     if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
       for (int t = 0; t < 8; ++t)
@@ -280,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_decode_kernel(cons
         float sum = 0.f, o = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float e = exp2_approx(stats[w][g][0] * kScaleLog2 - base);
+          const float e = part_weight(stats[w][g][0], base);
           sum += e * stats[w][g][1];
           o += e * merge[(w * group + g) * kMergeStride + threadIdx.x];
         }

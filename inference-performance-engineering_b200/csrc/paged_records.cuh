@@ -21,6 +21,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+constexpr float kTiny = 1.17549435e-38f;  // 2^-126, the least normal number, of bf16 too
+
+// What a part with maximum m counts beside `base` (of the largest one), at least kTiny: infinite values stay infinite.
+// A part without a key (m = -infinity) holds zeros.
+__device__ __forceinline__ float part_weight(float m, float base) { return fmaxf(exp2_approx(m * kScaleLog2 - base), kTiny); }
+
 // Units dealt to CTAs in contiguous runs, none of them without a unit and none with over one more than another.
 struct Deal {
   int runs, each, more;  // the first `more` runs have each + 1 units
@@ -99,13 +105,13 @@ __device__ __forceinline__ void join_parts(const Parts (&parts)[N], bf16* out) {
 #pragma unroll
       for (int k = 0; k < kTogether; ++k) most = fmaxf(most, m[k]);
       const float base = most == -INFINITY ? 0.f : most * kScaleLog2;
-      const float keep = exp2_approx(top * kScaleLog2 - base);
+      const float keep = part_weight(top, base);
       top = most;
       sum *= keep;
       o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
 #pragma unroll
       for (int k = 0; k < kTogether; ++k) {
-        const float e = exp2_approx(m[k] * kScaleLog2 - base);
+        const float e = part_weight(m[k], base);
         sum += e * l[k];
         o.x += e * x[k].x;
         o.y += e * x[k].y;

@@ -156,7 +156,8 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_norm: torch.Tensor, k_norm: t
 def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                            lengths: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """out [S, Hq * 128] = softmax(q k^T / sqrt(128)) v over keys 0 .. lengths[s] - 1 of every sequence, one query
-    token q [S, Hq, 128] each, 1 to 8 query heads per KV head. A sequence of length 0 gives zeros."""
+    token q [S, Hq, 128] each, 1 to 8 query heads per KV head. A sequence of length 0 gives zeros. An infinite value that
+    a row sees gives infinity, however small its weight (NaN beside one of the other sign, or where its score is -infinity)."""
     name = "paged_decode_attention"
     if _launched(nat.paged_calls().paged_decode_attention(q, k_pages, v_pages, page_table, lengths, out), name):
         return out

@@ -1,0 +1,118 @@
+"""What the attentions over a paged cache make of values that are not finite, against the definition.
+
+softmax(s) v with s = q k^T / sqrt(128), in 64 bits: a row that sees a score of +infinity or NaN is NaN throughout. A score of
+-infinity has the weight 0, which gives NaN beside a value that is not finite. Elsewhere a weight is above 0, however small,
+so an infinite value gives infinity, and NaN beside one of the other sign or a NaN.
+"""
+
+import math
+
+import pytest
+import torch
+
+from ipe_b200 import _native as nat
+from test_gpu_paged import DEV, HALF, NAN, Batch, decode, normal, prefill, shared
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def attend(batch, q):
+    """(o, A) of the definition in 64 bits [tokens, Hq * 128]; A = sum p |v| over the finite values."""
+    heads = q.shape[1]
+    o = torch.zeros(batch.tokens, heads, 128, dtype=torch.float64, device=DEV)
+    a = torch.zeros_like(o)
+    at = 0
+    for s, n in enumerate(batch.new):
+        total = batch.length[s]
+        for h in range(heads if total else 0):
+            k, v = batch.keys(s, h // (heads // batch.kv_heads), total)
+            score = q[at:at + n, h].double() @ k.T / math.sqrt(128)
+            hidden = torch.arange(total, device=DEV) > (total - n + torch.arange(n, device=DEV))[:, None]
+            score = torch.where(hidden, -INF, score)
+            p = torch.softmax(score, -1)
+            finite = torch.where(torch.isfinite(v), v, 0.0)
+            counted = (score > -INF).double()
+            nothing = (~hidden & (score == -INF)).double()
+            up, down = counted @ (v == INF).double() > 0, counted @ (v == -INF).double() > 0
+            none = (counted @ torch.isnan(v).double() + nothing @ (~torch.isfinite(v)).double() > 0) | (up & down)
+            x = torch.where(up, INF, p @ finite)
+            x = torch.where(down, -INF, x)
+            o[at:at + n, h] = torch.where(none | torch.isnan(p).any(-1, keepdim=True), NAN, x)
+            a[at:at + n, h] = p @ finite.abs()
+        at += n
+    return o.view(batch.tokens, -1), a.view(batch.tokens, -1)
+
+
+def check(out, batch, q):
+    """Equal where the definition is not finite; elsewhere the output's rounding, the weights' and the scores' (as in
+    test_gpu_paged.py)."""
+    o, a = attend(batch, q)
+    got = out[:batch.tokens].double()
+    lost = ~torch.isfinite(o)
+    assert torch.equal(torch.isnan(got), torch.isnan(o))
+    assert torch.equal(got == INF, o == INF) and torch.equal(got == -INF, o == -INF)
+    over = ((got - o).abs() - (HALF * o.abs() + (HALF + 2.0 ** -11) * a))[~lost]
+    assert over.numel() == 0 or float(over.max()) <= 0
+    assert nat.device_error() == 0
+
+
+def spoil(batch, seed):
+    """A few values of every sequence infinite or NaN, in dimensions of their own; the first and the last key's too."""
+    g = torch.Generator().manual_seed(seed)
+    for s, n in enumerate(batch.length):
+        if n == 0:
+            continue
+        for dim, value in ((0, INF), (1, -INF), (2, NAN), (3, INF), (3, -INF), (4, INF), (4, NAN), (5, INF), (6, -INF)):
+            key = {5: 0, 6: n - 1}.get(dim, int(torch.randint(n, (1,), generator=g)))
+            pages, rows = batch.places(s, key + 1, key)
+            batch.v[pages, :, rows, dim] = value
+    return batch
+
+
+DECODE = [
+    ([640], 16, 16, 8),
+    ([1, 16, 17, 63, 64, 65, 0, 300], 16, 4, 2),
+    ([5000, 1, 700], 64, 40, 8),
+    ([20000, 9], 32, 7, 1),
+    ([130] * 60, 128, 8, 8),
+]
+
+
+@pytest.mark.parametrize(("lengths", "page", "q_heads", "kv_heads"), DECODE)
+def test_decode_of_infinite_values(lengths, page, q_heads, kv_heads):
+    b = spoil(Batch([1] * len(lengths), [n - 1 for n in lengths], page, kv_heads, seed=7).fill(100), 8)
+    q = normal((len(lengths), q_heads, 128), 9, 1.5)
+    check(decode(b, q), b, q)
+
+
+@pytest.mark.parametrize("place", [0, 70, 299])
+@pytest.mark.parametrize("step", [1, 6])
+def test_decode_of_an_infinite_value_under_any_weight(place, step):
+    """Scores from about -150 to 150: an infinite value whose weight is the largest, one whose is below 1e-80, and between."""
+    b = Batch([1] * 2, [299, 40], 16, 2, seed=11).fill(200)
+    q = normal((2, 4, 128), 12, 4.0)
+    pages, rows = b.places(0)
+    direction = q[0].view(2, 2, 128).float().mean(1)
+    direction /= direction.norm(dim=-1, keepdim=True)
+    level = torch.linspace(-40, 40, 300, device=DEV)[torch.arange(300, device=DEV) * step * 49 % 300]
+    b.k[pages, :, rows] = (b.k[pages, :, rows].float() * 0.05 + level[:, None, None] * direction).bfloat16()
+    b.v[pages[place], :, rows[place], 3] = INF
+    b.v[pages[place], 1, rows[place], 4] = -INF
+    out = decode(b, q).view(2, 4, 128)
+    assert (out[0, :, 3] == INF).all() and (out[0, 2:, 4] == -INF).all()
+    bad = ~torch.isfinite(out)
+    assert int(bad.sum()) == 6
+    assert nat.device_error() == 0
+
+
+def test_decode_of_scores_that_are_not_finite():
+    """Keys with an infinite element: +infinity for some heads, -infinity (and the weight 0) for others."""
+    b = Batch([1] * 3, [299, 40, 700], 16, 2, seed=13).fill(300)
+    q = normal((3, 6, 128), 14, 1.5)
+    for s, key in ((0, 100), (1, 40), (2, 0)):
+        pages, rows = b.places(s, key + 1, key)
+        b.k[pages, :, rows, 9] = -INF
+        if s == 2:
+            b.v[pages, 0, rows, 5] = INF
+    check(decode(b, q), b, q)
