@@ -29,7 +29,8 @@
 //
 // Values past a block's last key are zeroed in shared memory before they meet their zero weights. A row
 // whose accumulator is not finite all the same (a value that is infinite or NaN, its own or one of a
-// later token in the tile) is computed again key by key from the keys it sees.
+// later token in the tile) is computed again from the keys it sees, when the CTA is done with its list of
+// work: no other row, and no wait, is behind it. A row that sees a score of infinity or NaN is NaN.
 // Every mbarrier wait is bounded; a timeout sets the device error word and the CTA winds down.
 #include <algorithm>
 
@@ -72,6 +73,7 @@ struct Shared {
   uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
   uint32_t tmem;
   int abort;
+  int again[8];  // by softmax warp: the list of rows that are attended again
   Work work[2];
   alignas(16) uint4 stage[8][32 * 4];  // by softmax warp
   int low[kMaxListed + 1], high[kMaxListed + 1];
@@ -229,33 +231,11 @@ __device__ __forceinline__ void exp2_pair(uint64_t x, float* p0, float* p1) {
   *p1 = __int_as_float((__float_as_int(n1) << 23) + __float_as_int(y1));
 }
 
-// A row key by key, by a whole warp: o (4 dimensions per lane), maximum and sum over keys [from, to).
-__device__ __forceinline__ void attend_row(const PagedCache& c, const bf16* q_row, const bf16* k, const bf16* v, int s,
-                                        int kv_head, int from, int to, float* o, float* top, float* sum) {
-  const int lane = threadIdx.x & 31;
-  const uint2 raw = ldcg8(q_row + lane * 4);
-  const float x[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16),
-                      __uint_as_float(raw.y & 0xffff0000u)};
-  float m = -INFINITY, l = 0.f;
-  o[0] = o[1] = o[2] = o[3] = 0.f;
-  for (int key = from; key < to; ++key) {
-    const int64_t at = (c.page_row(c.page(s, key), kv_head) + (key & (c.page_size() - 1))) * 128 + lane * 4;
-    const uint2 kr = ldcg8(k + at), vr = ldcg8(v + at);
-    float dot = x[0] * __uint_as_float(kr.x << 16) + x[1] * __uint_as_float(kr.x & 0xffff0000u) +
-                x[2] * __uint_as_float(kr.y << 16) + x[3] * __uint_as_float(kr.y & 0xffff0000u);
-    dot = warp_sum(dot);
-    const float next = fmaxf(m, dot), base = next == -INFINITY ? 0.f : next * kScaleLog2;
-    const float keep = exp2_approx(m * kScaleLog2 - base), p = exp2_approx(dot * kScaleLog2 - base);
-    m = next;
-    l = l * keep + p;
-    o[0] = o[0] * keep + p * __uint_as_float(vr.x << 16);
-    o[1] = o[1] * keep + p * __uint_as_float(vr.x & 0xffff0000u);
-    o[2] = o[2] * keep + p * __uint_as_float(vr.y << 16);
-    o[3] = o[3] * keep + p * __uint_as_float(vr.y & 0xffff0000u);
-  }
-  *top = m;
-  *sum = l;
-}
+// Which halves of two bf16 hold what, as 1 each.
+constexpr uint32_t kOnes = 0x3f803f80u, kInfinities = 0x7f807f80u;
+__device__ __forceinline__ uint32_t ones_where_infinite(uint32_t x, uint32_t sign) { return __vcmpeq2(x, kInfinities | sign) & kOnes; }
+__device__ __forceinline__ uint32_t ones_where_nan(uint32_t x) { return __vcmpgtu2(x & 0x7fff7fffu, kInfinities) & kOnes; }
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) { return __vcmpgeu2(x & 0x7fff7fffu, kInfinities); }
 
 // --------------------------------------------------------------------------- the list of work
 
@@ -323,6 +303,200 @@ __device__ __forceinline__ int last_at_most(const int* list, int n, int x) {
   return lo;
 }
 
+// Where a row goes unless to the output: `row` of a block's 256 in its record slot, or its own record.
+struct RecordPlace {
+  float* rec;  // null: to the output
+  bool part;
+  int m, sum;
+  __device__ __forceinline__ int vector(int v) const { return part ? block_vector(v) : v * 4; }
+};
+template <bool kShared>
+__device__ __forceinline__ RecordPlace record_place(const PrefillArgs& a, int record, int row, int64_t out_row) {
+  RecordPlace p;
+  p.part = record >= 0;
+  p.rec = p.part    ? a.records + static_cast<int64_t>(record) * kBlockRecord + row * 8
+          : kShared ? a.whole + out_row * kRecord
+                    : nullptr;
+  p.m = p.part ? kBlockRows * 128 - row * 7 : 128;
+  p.sum = p.part ? p.m + kBlockRows : 129;
+  return p;
+}
+
+// Rows of a softmax warp whose scores are finite and whose accumulators are not wait until the CTA's list of work has
+// ended, so that nothing waits for them. They make a list: what is known of a piece's rows stands in the place of the
+// first of them, which is named by its row of out or, where that is a part's, by ~(record slot * 256 + row).
+struct Again {
+  int token0, position0, sequence, kv_head, tile0, count;
+  unsigned rows;  // of the warp's 32
+  int next;
+};
+constexpr int kNoRow = INT32_MAX;
+template <bool kShared>
+__device__ __forceinline__ uint4* place_of_row(const PrefillArgs& a, int name) {
+  if (name < 0) return reinterpret_cast<uint4*>(a.records + static_cast<int64_t>(~name / kBlockRows) * kBlockRecord + ~name % kBlockRows * 8);
+  if (kShared) return reinterpret_cast<uint4*>(a.whole + static_cast<int64_t>(name) * kRecord);
+  return reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(name) * 128);
+}
+
+// The rows of one entry of that list, from the keys of their piece that each sees; gives the next entry's name. 16 rows
+// at a time, 16 keys a step, m16n8k16 products straight from the cache: 3 us a step, a chain of loads. (8192 tokens that
+// all see a NaN value: 4.7 ms instead of 0.25; a row of theirs alone would take as long key by key.) A value that is not
+// finite enters the products as 0; the rows that see it are found by products of 0 and 1 with where it is, and get
+// infinity, or NaN. The products' inner index is any order of the dimensions, and so are the values' columns: they are
+// such that a lane loads and stores 16 bytes at a time.
+template <bool kShared>
+__device__ __noinline__ int attend_again(const PrefillArgs& a, int name) {
+  const PagedCache& c = a.c;
+  const int lane = threadIdx.x & 31, g = lane >> 2, col = lane & 3, tile = threadIdx.x >> 7;
+  const int group = a.q_heads / c.kv_heads, per_tile = kBM / group;
+  const uint4* entry = place_of_row<kShared>(a, name);
+  const uint4 e0 = ldcg16(entry), e1 = ldcg16(entry + 1);
+  const Again w{static_cast<int>(e0.x), static_cast<int>(e0.y), static_cast<int>(e0.z), static_cast<int>(e0.w),
+                static_cast<int>(e1.x), static_cast<int>(e1.y), e1.z, static_cast<int>(e1.w)};
+  const int from = w.tile0 * kBN, to = from + w.count * kBN;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    const unsigned rows = w.rows >> (16 * half) & 0xffffu;
+    if (rows == 0) continue;
+    int number[2], lim[2];  // this lane's rows, g and g + 8 of the 16: as in the tile, and the keys they see
+    int64_t row[2];         // of q and out
+    uint4 q[2][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      number[r] = (threadIdx.x & 96) + half * 16 + g + 8 * r;
+      const int place = number[r] / group, token = tile * per_tile + place;
+      row[r] = static_cast<int64_t>(w.token0 + token) * a.q_heads + w.kv_head * group + number[r] - place * group;
+      lim[r] = 0;
+      if (rows >> (g + 8 * r) & 1) lim[r] = min(to, kShared ? c.length(w.token0 + token) : w.position0 + token + 1);
+      if (kShared) lim[r] = min(lim[r], a.shared_keys);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[r][i] = lim[r] > from ? ldcg16(a.q + row[r] * 128 + i * 32 + col * 8) : make_uint4(0, 0, 0, 0);
+    }
+    const int end = __reduce_max_sync(0xffffffffu, max(lim[0], lim[1]));
+    float o[16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll 1
+    for (int key0 = from; key0 < end; key0 += 16) {
+      const int64_t at = c.page_row(c.page(w.sequence, key0), w.kv_head) + (key0 & (c.page_size() - 1));  // 16 keys lie in a page
+      float s[2][4] = {};
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ldcg16(a.k + (at + 8 * t + g) * 128 + i * 32 + col * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          mma16816(s[t], q[0][i].x, q[1][i].x, q[0][i].y, q[1][i].y, x[i].x, x[i].y);
+          mma16816(s[t], q[0][i].z, q[1][i].z, q[0][i].w, q[1][i].w, x[i].z, x[i].w);
+        }
+      }
+      uint4 v[4][2];  // keys 2 col, 2 col + 1, and 8 on from these: dimensions 16 g .. 16 g + 15
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = 2 * col + (j & 1) + (j >> 1) * 8;
+        const bf16* vr = a.v + (at + key) * 128 + g * 16;
+        const bool seen = key0 + key < end;
+        v[j][0] = seen ? ldcg16(vr) : make_uint4(0, 0, 0, 0);
+        v[j][1] = seen ? ldcg16(vr + 8) : make_uint4(0, 0, 0, 0);
+      }
+      uint32_t p[4], counted[4], nothing[4];  // as fragments: weights, whether they are above 0, whether a seen key's is 0
+      float keep[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x[4], top = m[r];
+        bool seen[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          seen[e] = key0 + 8 * (e >> 1) + 2 * col + (e & 1) < lim[r];
+          x[e] = seen[e] ? s[e >> 1][2 * r + (e & 1)] : -INFINITY;
+          top = fmaxf(top, x[e]);
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float base = top == -INFINITY ? 0.f : top * kScaleLog2;
+        keep[r] = part_weight(m[r], base);
+        m[r] = top;
+        l[r] *= keep[r];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float p0 = exp2_approx(x[2 * t] * kScaleLog2 - base), p1 = exp2_approx(x[2 * t + 1] * kScaleLog2 - base);
+          l[r] += p0 + p1;
+          p[2 * t + r] = pack_bf16x2(p0, p1);
+          const uint32_t lo = seen[2 * t] ? 0x3f80u : 0u, hi = seen[2 * t + 1] ? 0x3f800000u : 0u;
+          const uint32_t lost = (x[2 * t] == -INFINITY ? 0xffffu : 0u) | (x[2 * t + 1] == -INFINITY ? 0xffff0000u : 0u);
+          counted[2 * t + r] = (lo | hi) & ~lost;
+          nothing[2 * t + r] = (lo | hi) & lost;
+        }
+      }
+      if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][e] *= keep[e >> 1];
+      }
+      uint32_t odd = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) odd |= not_finite(v[j][i].x) | not_finite(v[j][i].y) | not_finite(v[j][i].z) | not_finite(v[j][i].w);
+      const bool any_odd = __any_sync(0xffffffffu, odd != 0);
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        uint32_t b[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 &x = v[2 * j][t >> 3], &y = v[2 * j + 1][t >> 3];
+          const int word = t >> 1 & 3;
+          b[j] = __byte_perm(word == 0 ? x.x : word == 1 ? x.y : word == 2 ? x.z : x.w,
+                             word == 0 ? y.x : word == 1 ? y.y : word == 2 ? y.z : y.w, t & 1 ? 0x7632 : 0x5410);
+        }
+        if (any_odd) {
+          float up[4] = {}, down[4] = {}, none[4] = {};
+          mma16816(up, counted[0], counted[1], counted[2], counted[3], ones_where_infinite(b[0], 0u), ones_where_infinite(b[1], 0u));
+          mma16816(down, counted[0], counted[1], counted[2], counted[3], ones_where_infinite(b[0], 0x80008000u), ones_where_infinite(b[1], 0x80008000u));
+          mma16816(none, counted[0], counted[1], counted[2], counted[3], ones_where_nan(b[0]), ones_where_nan(b[1]));
+          mma16816(none, nothing[0], nothing[1], nothing[2], nothing[3], not_finite(b[0]) & kOnes, not_finite(b[1]) & kOnes);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (up[e] > 0.f) o[t][e] += INFINITY;
+            if (down[e] > 0.f) o[t][e] -= INFINITY;
+            if (none[e] > 0.f) o[t][e] = NAN;
+          }
+          b[0] &= ~not_finite(b[0]);
+          b[1] &= ~not_finite(b[1]);
+        }
+        mma16816(o[t], p[0], p[1], p[2], p[3], b[0], b[1]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (!(rows >> (g + 8 * r) & 1)) continue;
+      const RecordPlace at = record_place<kShared>(a, name < 0 ? ~name / kBlockRows : -1, tile * kBM + number[r], row[r]);
+      const float inv = lim[r] <= from ? 0.f : at.rec ? 1.f : 1.f / l[r];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // dimensions 32 col + 8 e on: of column 2 col, then of 2 col + 1
+        float f[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) f[d] = o[(e & 1) * 8 + d][2 * r + (e >> 1)] * inv;
+        if (at.rec) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+            *reinterpret_cast<float4*>(at.rec + at.vector(col * 8 + 2 * e + d)) = make_float4(f[4 * d], f[4 * d + 1], f[4 * d + 2], f[4 * d + 3]);
+        } else {
+          *reinterpret_cast<uint4*>(a.out + row[r] * 128 + col * 32 + e * 8) = pack8(f);
+        }
+      }
+      if (at.rec && col == 0) {
+        at.rec[at.m] = m[r];
+        at.rec[at.sum] = l[r];
+      }
+    }
+  }
+  __syncwarp();
+  return w.next;
+}
+
 // kShared: the "new tokens" are one query token of each sequence, all on the pages of c.prefix_pages (a
 // row sees those of them that its sequence's length covers), key tiles dealt in runs, and all rows go to
 // records that the decode kernel's merge joins with the rest of each sequence.
@@ -359,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.o_empty[i], 128);
     }
     sh.abort = 0;
+    for (int i = 0; i < 8; ++i) sh.again[i] = kNoRow;
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -855,15 +1030,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_after();
       const int64_t out_row = static_cast<int64_t>(w.token0 + token) * a.q_heads + w.kv_head * group + head;
-      // where the row goes unless to the output
-      const bool part = w.record >= 0;
-      const int record_row = i * kBM + r;
-      float* rec = part      ? a.records + static_cast<int64_t>(w.record) * kBlockRecord + record_row * 8
-                   : kShared ? a.whole + out_row * kRecord
-                             : nullptr;
-      const int at_m = part ? kBlockRows * 128 - record_row * 7 : 128, at_sum = part ? at_m + kBlockRows : 129;
+      const RecordPlace at = record_place<kShared>(a, w.record, i * kBM + r, out_row);
+      float* rec = at.rec;
       const bool sees = limit > w.tile0 * kBN;  // a key of this piece; else its weights are none
-      const float inv = !sees ? 0.f : rec ? 1.f : 1.f / l;
+      const float inv = odd ? NAN : !sees ? 0.f : rec ? 1.f : 1.f / l;  // scores that are not finite have no softmax
       float largest = 0.f;  // NaN if something is
       if (count > 0) {
         // Rows go out through shared memory, 64 bytes of 8 rows per store: 16 bytes of 32 rows each would
@@ -890,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (real) {
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(rec + (part ? block_vector(b * 8 + e) : (b * 8 + e) * 4)) =
+                *reinterpret_cast<float4*>(rec + at.vector(b * 8 + e)) =
                     make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
             }
           } else {
@@ -918,33 +1088,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < kD / 4; ++e) *reinterpret_cast<float4*>(rec + block_vector(e)) = make_float4(0.f, 0.f, 0.f, 0.f);
       }
       if (rec && real) {
-        rec[at_m] = m;
-        rec[at_sum] = sees ? l : 0.f;
+        rec[at.m] = m;
+        rec[at.sum] = odd ? NAN : sees ? l : 0.f;
       }
-      // rows with something not finite: again, key by key
-      unsigned again = __ballot_sync(0xffffffffu, real && count > 0 && (odd || !(largest <= 3.4e38f)));
-      __syncwarp();
-      while (__builtin_expect(again != 0, 0)) {
-        const int from = __ffs(again) - 1;
-        again &= again - 1;
-        const int64_t row = __shfl_sync(0xffffffffu, out_row, from);
-        const int keys = __shfl_sync(0xffffffffu, limit, from), first = w.tile0 * kBN;
-        float o[4], top, sum;
-        attend_row(c, a.q + row * 128, a.k, a.v, w.sequence, w.kv_head, first, min(keys, first + count * kBN), o, &top, &sum);
-        if (rec) {
-          float* at = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(rec), from));
-          *reinterpret_cast<float4*>(at + (part ? block_vector(lane) : lane * 4)) = make_float4(o[0], o[1], o[2], o[3]);
-          if (lane == from) {
-            rec[at_m] = top;
-            rec[at_sum] = sum;
-          }
-        } else {
-          const float s = keys > first ? 1.f / sum : 0.f;
-          *reinterpret_cast<uint2*>(a.out + row * 128 + lane * 4) =
-              make_uint2(pack_bf16x2(o[0] * s, o[1] * s), pack_bf16x2(o[2] * s, o[3] * s));
+      // rows with finite scores and something not finite
+      const unsigned again = __ballot_sync(0xffffffffu, real && count > 0 && !odd && !(largest <= 3.4e38f));
+      if (__builtin_expect(again != 0, 0)) {
+        __syncwarp();
+        if (lane == __ffs(again) - 1) {
+          const int name = at.part ? ~(w.record * kBlockRows + i * kBM + r) : static_cast<int>(out_row);
+          uint4* entry = place_of_row<kShared>(a, name);
+          entry[0] = make_uint4(w.token0, w.position0, w.sequence, w.kv_head);
+          entry[1] = make_uint4(w.tile0, count, again, sh.again[warp]);
+          sh.again[warp] = name;
         }
       }
     }
+    __syncwarp();
+    for (int name = sh.again[warp]; name != kNoRow;) name = attend_again<kShared>(a, name);
     if (!ok) *abort_flag = 1;
   }
 

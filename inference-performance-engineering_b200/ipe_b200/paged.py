@@ -180,7 +180,8 @@ def paged_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 def paged_prefill_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                             cu_tokens: torch.Tensor, lengths: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """Causal attention of ragged new tokens q [rows, Hq, 128] over their sequences' pages: token i of the n that
-    sequence s brings sees keys 0 .. lengths[s] - n + i. out [rows, Hq * 128]; 1 to 8 query heads per KV head."""
+    sequence s brings sees keys 0 .. lengths[s] - n + i. out [rows, Hq * 128]; 1 to 8 query heads per KV head. Infinite
+    values as in paged_decode_attention; rows that see values that are not finite take longer, behind all the others."""
     name = "paged_prefill_attention"
     if _launched(nat.paged_calls().paged_prefill_attention(q, k_pages, v_pages, page_table, cu_tokens, lengths, out), name):
         return out

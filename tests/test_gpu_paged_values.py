@@ -116,3 +116,97 @@ def test_decode_of_scores_that_are_not_finite():
         if s == 2:
             b.v[pages, 0, rows, 5] = INF
     check(decode(b, q), b, q)
+
+
+# ----------------------------------------------------------------------- prefill and the shared prefix
+
+PREFILL = [
+    ([1, 130], [0, 0], 16, 16, 8),
+    ([300, 17, 1, 0], [0, 900, 2000, 30], 64, 8, 2),
+    ([257], [0], 128, 5, 1),
+    ([100, 100], [129, 31], 16, 6, 2),
+    ([90], [5000], 32, 16, 8),
+    ([(37 * n) % 211 for n in range(40)], [(91 * n) % 517 for n in range(40)], 16, 24, 8),  # whole blocks, many per CTA
+]
+
+
+@pytest.mark.parametrize(("new", "past", "page", "q_heads", "kv_heads"), PREFILL)
+def test_prefill_of_infinite_values(new, past, page, q_heads, kv_heads):
+    b = spoil(Batch(new, past, page, kv_heads, seed=15).fill(400), 16)
+    q = normal((b.tokens, q_heads, 128), 17, 1.5)
+    out = prefill(b, q)
+    check(out, b, q)
+    assert torch.equal(torch.nan_to_num(out), torch.nan_to_num(prefill(b, q)))
+
+
+@pytest.mark.parametrize(("new", "past"), [([200, 70], [30, 500]), ([150] * 40, [20] * 40)])
+def test_prefill_of_scores_that_are_not_finite(new, past):
+    """A key with an infinite element early in every second sequence, under infinite values too; a NaN query."""
+    b = Batch(new, past, 16, 8, seed=18).fill(500)
+    q = normal((b.tokens, 16, 128), 19, 1.5)
+    for s in range(0, len(new), 2):
+        pages, rows = b.places(s, past[s] + 12, past[s] + 11)
+        b.k[pages, :, rows, 9] = -INF
+        b.v[pages, 0, rows, 5] = INF
+    q[new[0] // 2, 3] = NAN
+    check(prefill(b, q), b, q)
+
+
+SHARED = [
+    ([33, 40, 64], 2, 16, 16, 8),
+    ([32, 31, 1, 0, 33], 2, 16, 4, 2),
+    ([700 + 3 * n for n in range(20)], 40, 16, 16, 8),
+    ([1300 + n % 50 for n in range(130)], 20, 64, 40, 8),
+    ([513 + 128 * n for n in range(9)], 4, 128, 3, 1),
+    ([5000 - 70 * n for n in range(64)], 64, 64, 28, 4),
+]
+
+
+@pytest.mark.parametrize(("lengths", "prefix", "page", "q_heads", "kv_heads"), SHARED)
+def test_shared_prefix_of_infinite_values(lengths, prefix, page, q_heads, kv_heads):
+    b = spoil(Batch([1] * len(lengths), [n - 1 for n in lengths], page, kv_heads, seed=20, prefix=prefix).fill(600), 21)
+    q = normal((len(lengths), q_heads, 128), 22, 1.5)
+    check(shared(b, q), b, q)
+    b.page_table[:, :prefix] = b.prefix_pages
+    check(decode(b, q), b, q)
+    if min(lengths) > 0:  # a row of length 0 brings no token that prefill could place
+        check(prefill(b, q), b, q)
+
+
+# ------------------------------------------------------------------------------- a request gone wrong
+
+def milliseconds(call):
+    call()
+    torch.cuda.synchronize()
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    call()
+    end.record()
+    torch.cuda.synchronize()
+    return begin.elapsed_time(end)
+
+
+@pytest.mark.parametrize(("what", "most"), [("k", 2.0), ("q", 2.0), ("v", 40.0)])
+@pytest.mark.parametrize(("new", "past"), [([6000] + [100] * 20, [0] + [300] * 20), ([300, 60, 1], [9000, 2000, 4000])])
+def test_a_spoiled_request_does_not_hold_up_the_others(new, past, what, most):
+    """One NaN at the first position of a sequence, in whole blocks and in runs: the others' bits stay, and so does the
+    order of the call's time. NaN scores need no more work than others; a NaN value has the sequence's rows attended again
+    with the products of single warps. (Key by key, one row of 6000 keys took milliseconds, and there are 96000.)"""
+    n = new[0]
+    b = Batch(new, past, 64, 8, seed=23).fill(700)
+    q = normal((b.tokens, 16, 128), 24, 1.5)
+    good = prefill(b, q)
+    before = milliseconds(lambda: prefill(b, q))
+    pages, rows = b.places(0, 1)
+    if what == "q":
+        q[:n, :, 0] = NAN
+    else:
+        getattr(b, what)[pages, :, rows, 0] = NAN
+    out = prefill(b, q)
+    assert torch.equal(out[n:], good[n:])
+    lost = torch.isnan(out[:n].view(n, 16, 128))
+    assert lost[:, :, 0].all() and (what == "v" or lost.all())
+    if what == "v":
+        assert torch.equal(lost.sum(-1), torch.ones_like(lost[:, :, 0], dtype=torch.int64))
+    assert nat.device_error() == 0
+    assert milliseconds(lambda: prefill(b, q)) < most * before
