@@ -250,8 +250,8 @@ int ipe_prefill_attention(const void* q, const void* k_cache, const void* v_cach
  * outside [0, num_pages) device error 5; such a sequence's output rows hold no meaning, the others are served and
  * nothing outside the buffers is touched. Outputs must not overlap inputs. A page may stand in several rows of the
  * table, but not where two of them append: sequences that share a page only read it. Workspaces are 256-byte
- * aligned, as large as the _workspace function says on the device of the call, of any contents, and belong to the
- * call until it has run. */
+ * aligned, as large as the _workspace function says on the device of the call (0 for heads and pages that the call
+ * refuses), of any contents, and belong to the call until it has run. */
 
 /* ipe_qk_norm_rope_append (src/ipe/forward.py:101-109) for a ragged batch and a paged cache: token i of the n
  * that a sequence brings is at position lengths[s] - n + i. Computed in fp32 and rounded to bf16 once.

@@ -24,24 +24,31 @@ int finish(cudaError_t e, const char* name) {
   return e == cudaSuccess ? IPE_OK : fail(IPE_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
+bool heads_fit(int q_heads, int kv_heads) {
+  return q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && q_heads / kv_heads <= 8;
+}
+bool page_size_fits(int page_size) { return page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128; }
+// positions are 32-bit numbers in the kernels, and so is what they are rounded up to
+bool pages_fit(int pages, int page_size) { return pages <= (1 << 27) / page_size; }
+
 bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
 
 // The checks every paged entry point shares, and the kernels' view of the cache.
 int paged_cache(const char* name, const void* k_pages, const void* v_pages, const int32_t* page_table,
                 const int32_t* lengths, int64_t tokens, int sequences, int q_heads, int kv_heads, int64_t num_pages,
                 int page_size, int max_pages, ipe::PagedCache* c) {
-  if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || q_heads / kv_heads > 8)
+  if (!heads_fit(q_heads, kv_heads))
     return fail(IPE_ERR_UNSUPPORTED, "%s: %d query heads over %d KV heads: expected 1 to 8 query heads per KV head", name,
                 q_heads, kv_heads);
-  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+  if (!page_size_fits(page_size))
     return fail(IPE_ERR_UNSUPPORTED, "%s: page_size %d is not 16, 32, 64 or 128", name, page_size);
   if (tokens < 0 || sequences < 0 || num_pages < 1 || max_pages < 1)
     return fail(IPE_ERR_ARGUMENT, "%s: bad sizes (%lld rows, %d sequences, %lld pages, %d per sequence)", name,
                 static_cast<long long>(tokens), sequences, static_cast<long long>(num_pages), max_pages);
-  // positions, cache rows, (token, head) rows and units of 64 keys are 32-bit numbers in the kernels; their
-  // byte offsets are 64-bit
+  // cache rows, (token, head) rows and units of 64 keys are 32-bit numbers in the kernels too; their byte offsets
+  // are 64-bit
   if (tokens > INT32_MAX / q_heads || num_pages > INT32_MAX / (static_cast<int64_t>(kv_heads) * page_size) ||
-      max_pages > (1 << 27) / page_size || sequences > (1 << 24) ||
+      !pages_fit(max_pages, page_size) || sequences > (1 << 24) ||
       static_cast<int64_t>(sequences) * kv_heads > INT32_MAX / (static_cast<int64_t>(max_pages) * page_size / 64 + 1))
     return fail(IPE_ERR_UNSUPPORTED, "%s: sizes past the kernels' 32-bit row numbers", name);
   if (tokens == 0 || sequences == 0) return IPE_OK;
@@ -77,18 +84,20 @@ int workspace_checks(const char* name, const void* workspace, size_t bytes, size
 
 extern "C" {
 
+// Nothing for sizes that the entry points refuse: a caller allocates before it is told.
 size_t ipe_paged_decode_attention_workspace(int sequences, int q_heads, int kv_heads) {
-  if (sequences < 1 || kv_heads < 1 || q_heads < kv_heads) return 0;
+  if (sequences < 1 || !heads_fit(q_heads, kv_heads)) return 0;
   return ipe::paged_decode_workspace_bytes(sequences, q_heads, kv_heads);
 }
 
 size_t ipe_paged_prefill_attention_workspace(int64_t tokens, int sequences, int q_heads, int kv_heads) {
-  if (tokens < 1 || sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8) return 0;
+  if (tokens < 1 || sequences < 1 || !heads_fit(q_heads, kv_heads)) return 0;
   return ipe::paged_prefill_workspace_bytes(tokens, sequences, q_heads, kv_heads);
 }
 
 size_t ipe_shared_prefix_attention_workspace(int sequences, int q_heads, int kv_heads, int page_size, int prefix_count) {
-  if (sequences < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads / kv_heads > 8 || page_size < 1 || page_size > 128 || prefix_count < 0)
+  if (sequences < 1 || !heads_fit(q_heads, kv_heads) || !page_size_fits(page_size) || prefix_count < 0 ||
+      !pages_fit(prefix_count, page_size))
     return 0;
   ipe::PagedCache c{};
   c.sequences = sequences;

@@ -94,6 +94,19 @@ def test_no_workspace_for_pages_of_no_size():
         assert nat.load().ipe_shared_prefix_attention_workspace(4, 16, 8, page_size, 9) == 0
 
 
+@pytest.mark.parametrize(("q_heads", "kv_heads"), [(4096, 1), (9, 1), (15, 8), (8, 16), (0, 1), (16, 0), (-16, 8), (16, -8)])
+def test_no_workspace_for_heads_that_are_refused(q_heads, kv_heads):
+    lib = nat.load()
+    assert lib.ipe_paged_decode_attention_workspace(64, q_heads, kv_heads) == 0
+    assert lib.ipe_paged_prefill_attention_workspace(64, 2, q_heads, kv_heads) == 0
+    assert lib.ipe_shared_prefix_attention_workspace(64, q_heads, kv_heads, 16, 4) == 0
+
+
+@pytest.mark.parametrize(("page_size", "prefix_count"), [(24, 4), (1, 4), (8, 4), (128, 2 ** 20 + 1), (16, 2 ** 31 - 1), (64, -1)])
+def test_no_workspace_for_prefixes_that_are_refused(page_size, prefix_count):
+    assert nat.load().ipe_shared_prefix_attention_workspace(64, 16, 8, page_size, prefix_count) == 0
+
+
 def test_the_extension_module_leaves_other_calls_to_the_checks():
     x = torch.zeros(2, 2)
     calls = nat.paged_calls()
