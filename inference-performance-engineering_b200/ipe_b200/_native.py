@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import sysconfig
 from ctypes import c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 from types import ModuleType
@@ -148,12 +149,20 @@ def load() -> ctypes.CDLL:
 _calls: ModuleType | None = None
 
 
+def paged_calls_path() -> Path:
+    """Where the extension module for this interpreter and this torch is: it has their objects' layout compiled in, so one
+    that was built for others has another name and is never loaded."""
+    import torch
+
+    return LIBRARY.with_name(f"_paged_calls.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so")
+
+
 def paged_calls() -> ModuleType:
     """The extension module that launches the paged operators' ordinary calls (csrc/paged_calls.cpp)."""
     global _calls
     if _calls is None:
         load()
-        path = LIBRARY.with_name("_paged_calls.so")
+        path = paged_calls_path()
         spec = importlib.util.spec_from_file_location("_paged_calls", path)
         try:
             module = importlib.util.module_from_spec(spec)

@@ -5,7 +5,8 @@
 Each `csrc/*.cu` compiles to an object for `-gencode arch=compute_100a,code=sm_100a` (the only
 target: tcgen05 and TMA need the `a` variant), then one `-shared` link with the CUDA runtime linked
 statically. `csrc/paged_calls.cpp`, the Python functions of the paged operators, becomes the extension
-module `ipe_b200/lib/_paged_calls.so` beside it, against the torch that runs this. No JIT cache is used.
+module `ipe_b200/lib/_paged_calls.<interpreter>.torch-<version>.so` beside it, for the interpreter and the torch that
+run this. No JIT cache is used.
 """
 
 from __future__ import annotations
@@ -18,13 +19,14 @@ import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
+from ipe_b200 import _native
+
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent  # inference-performance-engineering_b200/
 CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB_DIR = PACKAGE / "lib"
 LIBRARY = LIB_DIR / "libipe_b200.so"
-CALLS = LIB_DIR / "_paged_calls.so"
 BUILD_DIR = ROOT / "_build"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -81,16 +83,16 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
 
 
 def build_calls(verbose: bool = False) -> Path:
-    source = CSRC / "paged_calls.cpp"
-    if not _stale(CALLS, [source, *INCLUDE.glob("*.h")]):
-        return CALLS
+    source, calls = CSRC / "paged_calls.cpp", _native.paged_calls_path()
+    if not _stale(calls, [source, *INCLUDE.glob("*.h")]):
+        return calls
     import torch
 
     torch_root = Path(torch.__file__).resolve().parent
     includes = [torch_root / "include", torch_root / "include" / "torch" / "csrc" / "api" / "include",
                 Path(nvcc()).resolve().parent.parent / "include", sysconfig.get_paths()["include"]]
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", *(f"-isystem{path}" for path in includes),
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(source), "-o", str(CALLS),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(source), "-o", str(calls),
            f"-L{torch_root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{LIB_DIR}", "-lipe_b200",
            "-Wl,-rpath,$ORIGIN"]
     if verbose:
@@ -98,7 +100,7 @@ def build_calls(verbose: bool = False) -> Path:
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError(f"g++ failed on {source.name}:\n{result.stderr}")
-    return CALLS
+    return calls
 
 
 if __name__ == "__main__":
