@@ -11,9 +11,10 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import sysconfig
+import warnings
 from ctypes import c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
-from types import ModuleType
+from types import ModuleType, SimpleNamespace
 
 LIBRARY = Path(__file__).resolve().parent / "lib" / "libipe_b200.so"
 
@@ -146,7 +147,7 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-_calls: ModuleType | None = None
+_calls: ModuleType | SimpleNamespace | None = None
 
 
 def paged_calls_path() -> Path:
@@ -157,8 +158,12 @@ def paged_calls_path() -> Path:
     return LIBRARY.with_name(f"_paged_calls.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so")
 
 
-def paged_calls() -> ModuleType:
-    """The extension module that launches the paged operators' ordinary calls (csrc/paged_calls.cpp)."""
+PAGED_CALLS = ("paged_qk_norm_rope_append", "paged_decode_attention", "paged_prefill_attention", "shared_prefix_attention")
+
+
+def paged_calls() -> ModuleType | SimpleNamespace:
+    """The extension module that launches the paged operators' ordinary calls (csrc/paged_calls.cpp). Without it (the
+    library alone was built) there is a warning, and a stand-in that takes no call: ipe_b200.paged launches them itself."""
     global _calls
     if _calls is None:
         load()
@@ -166,9 +171,11 @@ def paged_calls() -> ModuleType:
         spec = importlib.util.spec_from_file_location("_paged_calls", path)
         try:
             module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
         except ImportError as error:
-            raise NativeUnavailable(f"cannot load {path}: build it with `python -m ipe_b200.build` ({error})") from error
-        spec.loader.exec_module(module)
+            warnings.warn(f"{path.name} is not there or does not load: calls of the paged operators take the host longer "
+                          f"(`python -m ipe_b200.build` builds it; {error})", RuntimeWarning, stacklevel=3)
+            module = SimpleNamespace(**{name: lambda *args: None for name in PAGED_CALLS})
         _calls = module
     return _calls
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from ipe_b200 import _native as nat
-from ipe_b200 import build
+from ipe_b200 import build, ops
 
 
 @pytest.fixture
@@ -27,3 +27,46 @@ def test_a_module_of_another_torch_is_stale_and_not_loaded(unloaded, monkeypatch
 
 def test_the_module_of_this_torch_is_loaded(unloaded):
     assert nat.paged_calls().__spec__.origin == str(nat.paged_calls_path())
+
+
+@pytest.mark.parametrize("content", [None, b"", b"no module"])
+def test_without_a_module_the_operators_are_there(unloaded, monkeypatch, tmp_path, content):
+    path = tmp_path / "_paged_calls.so"
+    if content is not None:
+        path.write_bytes(content)
+    monkeypatch.setattr(nat, "paged_calls_path", lambda: path)
+    with pytest.warns(RuntimeWarning, match="_paged_calls"):
+        calls = nat.paged_calls()
+    assert all(getattr(calls, name)() is None for name in nat.PAGED_CALLS)
+    cpu = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):  # the checks of the Python functions are reached
+        ops.paged_decode_attention(cpu, cpu, cpu, cpu, cpu, cpu)
+
+
+@pytest.mark.gpu
+def test_without_a_module_the_results_are_the_same(unloaded, monkeypatch, tmp_path):
+    from test_gpu_paged import Batch, decode, normal, prefill, shared
+
+    b = Batch([1] * 3, [99, 40, 300], 16, 2, seed=1, prefix=2).fill(10)
+    q = normal((3, 4, 128), 2)
+    whole = b.page_table.clone()
+    whole[:, :2] = b.prefix_pages
+    qkv, w = normal((3, 8 * 128), 3), torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    cos, sin = normal((400, 128), 4), normal((400, 128), 5)
+
+    def outputs():
+        k, v, q_out = b.k.clone(), b.v.clone(), torch.zeros_like(q)
+        ops.paged_qk_norm_rope_append(qkv, w, w, cos, sin, b.cu, b.lengths, whole, 1e-6, q_out, k, v)
+        outs = [shared(b, q)]
+        b.page_table, table = whole, b.page_table
+        outs += [decode(b, q), prefill(b, q), q_out, k.nan_to_num(), v.nan_to_num()]
+        b.page_table = table
+        return outs
+
+    with_module = outputs()
+    monkeypatch.setattr(nat, "_calls", None)
+    monkeypatch.setattr(nat, "paged_calls_path", lambda: tmp_path / "_paged_calls.so")
+    with pytest.warns(RuntimeWarning, match="_paged_calls"):
+        without = outputs()
+    assert all(torch.equal(x, y) for x, y in zip(with_module, without))
+    assert nat.device_error() == 0
