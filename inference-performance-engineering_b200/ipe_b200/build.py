@@ -16,6 +16,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -82,16 +83,24 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     return LIBRARY
 
 
-def build_calls(verbose: bool = False) -> Path:
+def build_calls(verbose: bool = False) -> Path | None:
+    """The extension module, or None, with a warning, where a compiler or headers for it are missing: the library needs
+    neither, and the operators run without the module."""
     source, calls = CSRC / "paged_calls.cpp", _native.paged_calls_path()
     if not _stale(calls, [source, *INCLUDE.glob("*.h")]):
         return calls
     import torch
 
     torch_root = Path(torch.__file__).resolve().parent
+    python_include, compiler = Path(sysconfig.get_paths()["include"]), shutil.which("g++")
+    missing = [str(path) for path in (python_include / "Python.h", torch_root / "include" / "ATen" / "ATen.h") if not path.exists()]
+    if missing or compiler is None:
+        warnings.warn(f"{calls.name} is not built, for want of {', '.join(missing or ['g++'])}: the library is complete "
+                      "without it", RuntimeWarning, stacklevel=2)
+        return None
     includes = [torch_root / "include", torch_root / "include" / "torch" / "csrc" / "api" / "include",
-                Path(nvcc()).resolve().parent.parent / "include", sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", *(f"-isystem{path}" for path in includes),
+                Path(nvcc()).resolve().parent.parent / "include", python_include]
+    cmd = [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", *(f"-isystem{path}" for path in includes),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", str(source), "-o", str(calls),
            f"-L{torch_root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", f"-L{LIB_DIR}", "-lipe_b200",
            "-Wl,-rpath,$ORIGIN"]

@@ -43,6 +43,19 @@ def test_without_a_module_the_operators_are_there(unloaded, monkeypatch, tmp_pat
         ops.paged_decode_attention(cpu, cpu, cpu, cpu, cpu, cpu)
 
 
+@pytest.mark.parametrize("missing", ["g++", "Python.h"])
+def test_the_library_is_built_where_the_module_cannot_be(monkeypatch, tmp_path, missing):
+    find, paths = build.shutil.which, build.sysconfig.get_paths
+    monkeypatch.setattr(nat, "paged_calls_path", lambda: tmp_path / "_paged_calls.so")
+    if missing == "g++":
+        monkeypatch.setattr(build.shutil, "which", lambda name: None if name == "g++" else find(name))
+    else:
+        monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {**paths(), "include": str(tmp_path)})
+    with pytest.warns(RuntimeWarning, match=r"g\+\+" if missing == "g++" else "Python.h"):
+        assert build.build() == build.LIBRARY
+    assert not (tmp_path / "_paged_calls.so").exists()
+
+
 @pytest.mark.gpu
 def test_without_a_module_the_results_are_the_same(unloaded, monkeypatch, tmp_path):
     from test_gpu_paged import Batch, decode, normal, prefill, shared
