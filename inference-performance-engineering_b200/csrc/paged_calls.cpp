@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "ipe_b200.h"
@@ -89,12 +90,9 @@ PyObject* guarded(Py_ssize_t given, Py_ssize_t expected, Body&& body) {
     PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", expected, given);
     return nullptr;
   }
-  try {
-    return body();
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS  // what torch throws (a workspace that does not fit the device's memory) as torch raises it
+  return body();
+  END_HANDLE_TH_ERRORS
 }
 
 // (qkv, q_norm, k_norm, cos, sin, cu_tokens, lengths, page_table, eps, q_out, k_pages, v_pages)

@@ -1,5 +1,6 @@
 """The extension module behind the paged operators' Python functions: which file is loaded, without a GPU."""
 
+import contextlib
 import sysconfig
 
 import pytest
@@ -83,3 +84,24 @@ def test_without_a_module_the_results_are_the_same(unloaded, monkeypatch, tmp_pa
         without = outputs()
     assert all(torch.equal(x, y) for x, y in zip(with_module, without))
     assert nat.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("module", [True, False])
+def test_a_workspace_that_does_not_fit_is_out_of_memory(unloaded, monkeypatch, tmp_path, module):
+    if not module:
+        monkeypatch.setattr(nat, "paged_calls_path", lambda: tmp_path / "_paged_calls.so")
+    from test_gpu_paged import DEV
+
+    pages = torch.zeros(1, 8, 16, 128, dtype=torch.bfloat16, device=DEV)
+    q = torch.zeros(64, 64, 128, dtype=torch.bfloat16, device=DEV)
+    table, lengths = torch.zeros(64, 1, dtype=torch.int32, device=DEV), torch.zeros(64, dtype=torch.int32, device=DEV)
+    out = torch.zeros(64, 64 * 128, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(1e-6)
+    try:
+        with pytest.warns(RuntimeWarning) if not module else contextlib.nullcontext(), pytest.raises(torch.OutOfMemoryError):
+            ops.paged_decode_attention(q, pages, pages, table, lengths, out)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert (ops.paged_decode_attention(q, pages, pages, table, lengths, out) == 0).all()
