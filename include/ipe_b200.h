@@ -248,7 +248,8 @@ int ipe_prefill_attention(const void* q, const void* k_cache, const void* v_cach
  * The integers are read on the device only, so a captured call replays with other values. A length that is
  * negative, larger than max_pages * page_size or less than the sequence's new tokens sets device error 2, a page
  * outside [0, num_pages) device error 5; such a sequence's output rows hold no meaning, the others are served and
- * nothing outside the buffers is touched. Outputs must not overlap inputs. A page may stand in several rows of the
+ * nothing outside the buffers is touched. Offsets that are not ascending rows set device error 2 in the attention, which
+ * serves the sequences before the first such one. Outputs must not overlap inputs. A page may stand in several rows of the
  * table, but not where two of them append: sequences that share a page only read it. Workspaces are 256-byte
  * aligned, as large as the _workspace function says on the device of the call (0 for heads and pages that the call
  * refuses), of any contents, and belong to the call until it has run. */

@@ -239,14 +239,15 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t x) { return __vcmpgeu2(x
 
 // --------------------------------------------------------------------------- the list of work
 
-// A sequence's new tokens [begin, end) of q's rows, and its length; no tokens where the offsets are none.
+// A sequence's new tokens [begin, end) of q's rows, and its length, -1 where the offsets are none. The list ends before
+// the first such sequence: the offsets of those before it ascend, so no row belongs to two of them.
 struct Span {
   int begin, tokens, length;
 };
 __device__ __forceinline__ Span span_from(const PagedCache& c, int rows, int b, int e, int n) {
   if (b < 0 || e < b || e > rows) {
     report(c.err, kErrPositionRange);
-    return Span{0, 0, 0};
+    return Span{0, 0, -1};
   }
   const int length = c.checked_length(n);
   if (e - b > length) report(c.err, kErrPositionRange);
@@ -324,7 +325,8 @@ __device__ __forceinline__ RecordPlace record_place(const PrefillArgs& a, int re
 
 // Rows of a softmax warp whose scores are finite and whose accumulators are not wait until the CTA's list of work has
 // ended, so that nothing waits for them. They make a list: what is known of a piece's rows stands in the place of the
-// first of them, which is named by its row of out or, where that is a part's, by ~(record slot * 256 + row).
+// first of them (no row is another piece's), which is named by its row of out or, where that is a part's, by
+// ~(record slot * 256 + row).
 struct Again {
   int token0, position0, sequence, kv_head, tile0, count;
   unsigned rows;  // of the warp's 32
@@ -566,6 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int shared_tiles = (a.shared_keys + kBN - 1) / kBN;
       int blocks = 0, tiles = 0, most = 0;
       bool whole = false;
+      int sound = c.sequences;         // sequences before the first whose offsets are none
       Span mine{0, 0, 0};            // of sequence `lane`
       int mine_first = 0, mine_n = 0;  // its blocks among all
       auto span_at = [&](int s) {  // of any, for a whole warp
@@ -580,7 +583,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int base = 0; base < c.sequences; base += 32) {
           const int s = base + lane;
           Span x{0, 0, 0};
-          if (s < c.sequences) x = base == 0 ? span_from(c, a.tokens, first[0], first[1], first[2]) : span_of(c, s, a.tokens);
+          if (s < sound) x = base == 0 ? span_from(c, a.tokens, first[0], first[1], first[2]) : span_of(c, s, a.tokens);
+          const unsigned none = __ballot_sync(0xffffffffu, x.length < 0);
+          if (none != 0) sound = base + __ffs(none) - 1;
+          if (s >= sound) x = Span{0, 0, 0};
           const int n = (x.tokens + per_block - 1) / per_block, low = max(0, x.length - x.tokens) / per_block;
           const int before = blocks + warp_scan(n);
           if (base == 0) {
@@ -630,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool listed = c.sequences <= kMaxListed;
       auto range_of = [&](int s, int* low, int* high) {
         *low = *high = 0;
-        if (s >= c.sequences) return;
+        if (s >= sound) return;
         if (listed) {
           *low = sh.low[s];
           *high = sh.high[s];
@@ -951,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int limit = 0;  // keys the row sees
       if (real) limit = kShared ? min(c.length(w.token0 + token), a.shared_keys) : max(0, w.position0 + token + 1);
       float m = -INFINITY, l = 0.f;
-      bool odd = false;  // scores that are infinite or not a number
+      bool odd = false;  // scores that are infinite or not a number: there is no softmax
       for (int step = 0; step < count && ok; ++step) {
         if (!wait_all(&sh.s_full[i], s_seen & 1)) {
           ok = false;
@@ -1033,7 +1039,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const RecordPlace at = record_place<kShared>(a, w.record, i * kBM + r, out_row);
       float* rec = at.rec;
       const bool sees = limit > w.tile0 * kBN;  // a key of this piece; else its weights are none
-      const float inv = odd ? NAN : !sees ? 0.f : rec ? 1.f : 1.f / l;  // scores that are not finite have no softmax
+      const float inv = odd ? NAN : !sees ? 0.f : rec ? 1.f : 1.f / l;
       float largest = 0.f;  // NaN if something is
       if (count > 0) {
         // Rows go out through shared memory, 64 bytes of 8 rows per store: 16 bytes of 32 rows each would

@@ -13,7 +13,8 @@ synchronises, and replays from a CUDA graph with other values in them. What only
 checks there (`ipe_b200._native.device_error`): a length that is negative, too long for its row of the
 page table or less than the sequence's new tokens sets device error 2, a page outside the cache device
 error 5. Keys without a place are not appended and such a sequence's output rows hold no meaning; the other
-sequences are served, and nothing outside the tensors is touched.
+sequences are served, and nothing outside the tensors is touched. Offsets that are not ascending rows set device error 2
+in paged_prefill_attention, which serves the sequences before the first such one.
 
 Every function runs on the current stream of its tensors' device. Outputs must not overlap inputs.
 

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from ipe_b200 import _native as nat
+from ipe_b200 import ops
 from test_gpu_paged import DEV, HALF, NAN, Batch, decode, normal, prefill, shared
 
 pytestmark = pytest.mark.gpu
@@ -210,3 +211,26 @@ def test_a_spoiled_request_does_not_hold_up_the_others(new, past, what, most):
         assert torch.equal(lost.sum(-1), torch.ones_like(lost[:, :, 0], dtype=torch.int64))
     assert nat.device_error() == 0
     assert milliseconds(lambda: prefill(b, q)) < most * before
+
+
+@pytest.mark.parametrize(("cu", "sequences"), [
+    ([0, 60, 0, 60, 100], 4), ([0, 60, 50, 60, 100], 4), ([0, 60, 90, 30, 100], 4), ([0, 60, 2 ** 30, 30, 60], 4), ([0, 0, -60, 0, 60], 4),
+    ([0, 60, 0, 60, 100], 40), ([0, 60, 90, 30, 100], 1100)])
+def test_prefill_offsets_that_are_no_offsets(cu, sequences):
+    """Offsets that do not ascend, over values that are not finite: the sequences before are served, the rows of the others
+    are left as they are, and so is what lies around the output."""
+    sound = next(s for s in range(4) if not 0 <= cu[s] <= cu[s + 1] <= 100)
+    b = spoil(Batch([60] + [40] * (sequences - 1), [300] * sequences, 16, 2, seed=25).fill(800), 26)
+    q = normal((100, 4, 128), 27, 1.5)
+    b.cu = torch.tensor(cu + [100] * (sequences - 4), dtype=torch.int32, device=DEV)
+    guarded = torch.full((100 + 64, 512), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = guarded[32:132]
+    for _ in range(3):
+        ops.paged_prefill_attention(q, b.k, b.v, b.page_table, b.cu, b.lengths, out)
+        assert nat.device_error() == 2
+    assert (guarded[:32] == 7).all() and (guarded[132:] == 7).all()
+    served = cu[sound] if sound else 0
+    b.new, b.tokens = [cu[i + 1] - cu[i] for i in range(sound)], served
+    if served:
+        check(out, b, q[:served])
+    assert (out[served:] == 7).all()
