@@ -95,13 +95,20 @@ def test_a_workspace_that_does_not_fit_is_out_of_memory(unloaded, monkeypatch, t
 
     pages = torch.zeros(1, 8, 16, 128, dtype=torch.bfloat16, device=DEV)
     q = torch.zeros(64, 64, 128, dtype=torch.bfloat16, device=DEV)
-    table, lengths = torch.zeros(64, 1, dtype=torch.int32, device=DEV), torch.zeros(64, dtype=torch.int32, device=DEV)
-    out = torch.zeros(64, 64 * 128, dtype=torch.bfloat16, device=DEV)
+    table, lengths = torch.zeros(64, 100, dtype=torch.int32, device=DEV), torch.zeros(64, dtype=torch.int32, device=DEV)
+    prefix, out = torch.zeros(100, dtype=torch.int32, device=DEV), torch.ones(64, 64 * 128, dtype=torch.bfloat16, device=DEV)
+    need, held = nat.load().ipe_shared_prefix_attention_workspace(64, 64, 8, 16, 100), []
     torch.cuda.empty_cache()
     torch.cuda.set_per_process_memory_fraction(1e-6)
     try:
+        with pytest.raises(torch.OutOfMemoryError):
+            while True:  # what the allocator has left over in blocks that it cannot give back
+                held.append(torch.empty(need, dtype=torch.uint8, device=DEV))
         with pytest.warns(RuntimeWarning) if not module else contextlib.nullcontext(), pytest.raises(torch.OutOfMemoryError):
-            ops.paged_decode_attention(q, pages, pages, table, lengths, out)
+            ops.shared_prefix_attention(q, pages, pages, prefix, table, lengths, out)
     finally:
+        held.clear()
         torch.cuda.set_per_process_memory_fraction(1.0)
-    assert (ops.paged_decode_attention(q, pages, pages, table, lengths, out) == 0).all()
+    assert (out == 1).all()
+    ops.shared_prefix_attention(q, pages, pages, prefix, table, lengths, out)
+    assert (out == 0).all()
