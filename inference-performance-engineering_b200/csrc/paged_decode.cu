@@ -12,11 +12,13 @@
 // belong to the same two heads. P enters as two bf16 terms (the value cut off and the remainder), so the
 // weights keep 16 bits: the products are idle anyway. Neither term of a key with a finite score is ever
 // 0 or negative, nor a factor that rescales what came before 0 (kTiny is the least of them): an infinite
-// value that a row sees stays infinite, with its sign, however small its weight. What a warp waits for (its loads, the chain from scores to weights)
-// the other warps of the SM fill: 3 CTAs with 2 units in flight each against 2 with 3 measured 101.5 and
-// 110.8 us for 160 rows behind a shared prefix, 111.0 and 114.8 for 64 rows of 700 to 12289 keys (6.1 TB/s).
-// 16 rows of 90 to 30001 keys: 57.7 us, 5.2 TB/s, of which the start and the merge take 8; one row of 640
-// keys: 5.8 us, two launches and their chains of loads.
+// value that a row sees stays infinite, with its sign, however small its weight. What a warp waits for (its
+// loads, the chain from scores to weights) the other warps of the SM fill: 3 CTAs with 2 units in flight each
+// against 2 with 3 measured 101.5 and 110.8 us for 160 rows behind a shared prefix, 111.0 and 114.8 for 64 rows
+// of 700 to 12289 keys, in captured graphs. Measured, called alone behind a flush of L2, and as a share of a
+// captured graph of 12 calls: those 64 rows 115.6 and 112.1 us (5.8 and 6.0 TB/s); 16 rows of 90 to 30001 keys
+// 59.9 and 57.8 us (5.1 and 5.2 TB/s), of which the start and the merge take 8; one row of 640 keys 8.2 and
+// 5.9 us, two launches and their chains of loads.
 // K and V come through per-warp rings of cp.async copies, which fill keys past the sequence's end with zeros
 // without reading them: what an unused row holds (NaN, say) never meets a weight of zero.
 #include <algorithm>

@@ -14,18 +14,23 @@
 //
 // Bound, on long prompts, by the chain of a tile: a step (128 keys of both query tiles) is 2070 cycles of
 // products and takes about 2950, with the scores' way through the softmax warps (1400 cycles per tile, the
-// special function unit half busy) and back between two products of the same tile. 8192 new tokens, 16 query
-// heads over 8: 217 us, 1260 TFLOP/s of the products below the diagonal (0.77 of the measured peak). Nine
-// prompts of 17 to 2500 tokens, 32 heads over 8: 115 us, 980 TFLOP/s; there the change from one piece to the
+// special function unit half busy) and back between two products of the same tile. Measured, called alone behind a
+// flush of L2, and as a share of a captured graph of 12 calls: 8192 new tokens, 16 query heads over 8, 253 and 225 us,
+// 1090 and 1220 TFLOP/s of the products below the diagonal (0.66 and 0.74 of the measured peak). Nine prompts of
+// 17 to 2500 tokens, 32 heads over 8, 136 and 115 us, 830 and 980 TFLOP/s; there the change from one piece to the
 // next counts, 6000 cycles beside a step's. Much of them is instruction fetch, so what runs once per piece stands
-// in rolled loops (119 us with them unrolled). Pieces of two prompts on 9000 to 20000 cached tokens: 57 to 68
-// us, about 2 TB/s. 512 tokens: 15 us, a chain of lookups and four steps.
+// in rolled loops (in the graph 119 us with them unrolled). Pieces of two prompts on 9000 to 20000 cached tokens: 62
+// and 57 to 68 us, about 2 TB/s. 512 tokens: 16.4 and 15.5 us, a chain of lookups and four steps.
 //
 // Warps 0-3 and 4-7: softmax of query tile 0 and 1, one row per thread; warp 8: work list and TMA loads;
 // warp 9: tensor memory and MMA issue. Persistent, one CTA per SM; the blocks go to the CTAs heaviest
 // first, back and forth. Where there are fewer blocks than that can balance (two per SM), every block's key
 // tiles are dealt to the CTAs in equal contiguous runs instead; parts of a block go to the workspace as
-// records (unnormalised o, maximum, sum), merged by a second kernel in order of the keys.
+// records (unnormalised o, maximum, sum), merged by a second kernel in order of the keys. The host decides
+// between the two by the sizes it sees, rows behind the last sequence among them, not by the lengths: many
+// sequences, or a buffer much larger than its tokens, leave a long context to one CTA per block. (One new token
+// each of 36 and of 40 sequences, one of them on 30000 keys, 16 heads over 8: 106 and 446 us. Two pieces on 9000
+// and 20000 keys, no, 4000 and 4800 rows behind them: 79, 87 and 311 us.)
 //
 // Values past a block's last key are zeroed in shared memory before they meet their zero weights. A row
 // whose accumulator is not finite all the same (a value that is infinite or NaN, its own or one of a
@@ -1123,7 +1128,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The blocks whose key tiles lie in more than one run: a CTA per (block, KV head, 8 rows), a warp per row.
+// The blocks whose key tiles lie in more than one run: a CTA per (block, KV head, 4 rows), a warp per row.
 constexpr int kMergeRows = 4;
 __global__ void __launch_bounds__(kMergeRows * 32) paged_prefill_merge_kernel(const PrefillArgs a, int ctas) {
   const int block = blockIdx.x / a.c.kv_heads, kv_head = blockIdx.x - block * a.c.kv_heads;

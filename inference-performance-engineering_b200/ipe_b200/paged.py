@@ -16,6 +16,7 @@ error 5. Keys without a place are not appended and such a sequence's output rows
 sequences are served, and nothing outside the tensors is touched. Offsets that are not ascending rows set device error 2
 in paged_prefill_attention, which serves the sequences before the first such one.
 
+Scores, weighted sums of values and their sums of weights are fp32; sums that pass its range are infinite.
 Every function runs on the current stream of its tensors' device. Outputs must not overlap inputs.
 
   paged_qk_norm_rope_append   q/k norm, rotation and the append (src/ipe/forward.py:101-109)
