@@ -182,3 +182,15 @@ def test_decode_of_rising_scores(lengths, page, q_heads, kv_heads):
     b, direction = rising(Batch([1] * len(lengths), [n - 1 for n in lengths], page, kv_heads, seed=6), 50)
     q = follow(b, direction, q_heads, 60)
     check_moves(decode(b, q), b, q)
+
+
+@pytest.mark.parametrize(("new", "past", "page", "q_heads", "kv_heads"), [([900], [0], 16, 4, 2), ([70, 9, 1], [3000, 900, 700], 32, 16, 8)])
+def test_prefill_of_rising_scores_and_large_values(new, past, page, q_heads, kv_heads):
+    """Values of about 2^116: weights of up to 256 beside a maximum that has not moved take the accumulators past fp32's
+    range, weights of at most 1 do not."""
+    b, direction = rising(Batch(new, past, page, kv_heads, seed=7), 70, most=3)
+    b.v *= 2.0 ** 116
+    q = follow(b, direction, q_heads, 80)
+    out = prefill(b, q)
+    assert torch.isfinite(out).all()
+    check_moves(out, b, q)
